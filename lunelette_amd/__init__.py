@@ -2,9 +2,9 @@
 
 The product is the C-ABI shared library lunelette_amd/liblunelette_hip.so
 (include/lunelette_runtime.h, include/lunelette_kernels.h,
-include/lunelette_generation.h, include/lunelette_session.h,
-include/lunelette_artifacts.h, include/lunelette_tokenizer.h,
-include/lunelette_chat.h). This module only loads it and declares
+include/lunelette_serving.h, include/lunelette_generation.h,
+include/lunelette_session.h, include/lunelette_artifacts.h,
+include/lunelette_tokenizer.h, include/lunelette_chat.h). This module only loads it and declares
 prototypes; it never substitutes another implementation. If the library has
 not been built, `lib()` raises.
 """
@@ -35,6 +35,8 @@ COMPACT_FP8_LOOKUP = 2
 
 PATH_FUSED, PATH_LOOKUP, PATH_UNFUSED, PATH_RESIDENT, PATH_MFMA = range(5)
 OP_QKV_ROPE, OP_ATTENTION, OP_O_RESIDUAL, OP_GATEUP_SILU, OP_DOWN_RESIDUAL = range(5)
+CACHE_F16, CACHE_Q4 = range(2)
+LOGPROBS_TOP = 64
 
 _lib = None
 _test_lib = None
@@ -68,6 +70,21 @@ class LayerWeights(ctypes.Structure):
                 ("f32_qkv", c_void), ("f32_o", c_void), ("f32_gate", c_void), ("f32_up", c_void),
                 ("f32_down", c_void), ("scale", ctypes.c_float * 7),
                 ("input_norm", c_void), ("post_norm", c_void)]
+
+
+class PagedCache(ctypes.Structure):
+    """lh_paged_cache."""
+    _fields_ = [("kind", ctypes.c_int), ("kv_heads", ctypes.c_uint32),
+                ("head_dim", ctypes.c_uint32), ("page_size", ctypes.c_uint32),
+                ("pages", ctypes.c_uint32), ("data", c_void)]
+
+
+class PagedBatch(ctypes.Structure):
+    """lh_paged_batch."""
+    _fields_ = [("sequences", ctypes.c_uint32), ("tokens", ctypes.c_uint32),
+                ("table_width", ctypes.c_uint32), ("max_query", ctypes.c_uint32),
+                ("max_length", ctypes.c_uint32), ("query_start", c_void), ("length", c_void),
+                ("table", c_void)]
 
 
 class GenerationConfig(ctypes.Structure):
@@ -210,10 +227,31 @@ def _load(path):
     _proto(l, "lunelette_generate_with_logits_capacity", i, LOGITS_FN, c_void, c_int64_p, c_size,
            c_size, ctypes.POINTER(GenerationConfig), ctypes.POINTER(GenerationResult), err,
            c_size)
+    declare_serving(l)
     declare_session(l)
     declare_artifacts(l)
     declare_tokenizer(l)
     return l
+
+
+def declare_serving(l):
+    """Prototypes of include/lunelette_serving.h on a loaded library."""
+    i, f, u, p = ctypes.c_int, ctypes.c_float, ctypes.c_uint32, c_void
+    cache, batch = ctypes.POINTER(PagedCache), ctypes.POINTER(PagedBatch)
+    _proto(l, "lh_q4_bytes", c_size, c_size, c_size, c_size)
+    _proto(l, "lh_q4_pack", i, p, p, c_size, c_size, c_size, p, p)
+    _proto(l, "lh_q4_quantize", i, p, c_size, c_size, c_size, p, p)
+    _proto(l, "lh_q4_scratch", c_size, c_size, c_size)
+    _proto(l, "lh_q4_matvec", i, p, p, c_size, p, c_size, c_size, c_size, c_size, c_size, p,
+           c_size, p)
+    _proto(l, "lh_logprobs_scratch", c_size, c_size, c_size, c_size)
+    _proto(l, "lh_logprobs", i, p, c_size, c_size, c_size, p, p, p, c_size, p, p, p, c_size, p)
+    _proto(l, "lh_paged_cache_bytes", c_size, cache)
+    _proto(l, "lh_paged_append", i, cache, batch, u, p, c_size, p, c_size, p, c_size, p, p, u, p,
+           p, c_size, p)
+    _proto(l, "lh_paged_read", i, cache, batch, p, c_size, p, c_size, p)
+    _proto(l, "lh_paged_attention_scratch", c_size, cache, batch, u)
+    _proto(l, "lh_paged_attention", i, cache, batch, u, p, c_size, f, p, c_size, p, c_size, p)
 
 
 class SessionWork(ctypes.Structure):

@@ -32,6 +32,13 @@ __device__ __forceinline__ float bf16_to_f32(uint32_t bits16)
     return __uint_as_float(bits16 << 16);
 }
 
+// BF16 nearest to a finite v, ties to even (Inf past the largest).
+__device__ __forceinline__ uint32_t bf16_nearest(float v)
+{
+    const uint32_t u = __float_as_uint(v);
+    return (u + 0x7fffu + ((u >> 16) & 1)) >> 16;
+}
+
 // Pairwise halving tree over the 64 lanes of a wave: after the step with
 // distance s, lane i < s holds v_i + v_{i+s}; lane 0 returns the total.
 // Distances 32 and 16 use gfx950's v_permlane32_swap / v_permlane16_swap,
