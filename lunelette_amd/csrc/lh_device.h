@@ -39,6 +39,15 @@ __device__ __forceinline__ uint32_t bf16_nearest(float v)
     return (u + 0x7fffu + ((u >> 16) & 1)) >> 16;
 }
 
+// Four floats from any 4-byte boundary: one 16-byte load, which this chip takes from
+// there (a wave's contiguous words then touch one cache line more).
+__device__ __forceinline__ float4 load4(const float* p)
+{
+    typedef float float4_any __attribute__((ext_vector_type(4), aligned(4)));
+    const float4_any v = *reinterpret_cast<const float4_any*>(p);
+    return make_float4(v.x, v.y, v.z, v.w);
+}
+
 // Pairwise halving tree over the 64 lanes of a wave: after the step with
 // distance s, lane i < s holds v_i + v_{i+s}; lane 0 returns the total.
 // Distances 32 and 16 use gfx950's v_permlane32_swap / v_permlane16_swap,

@@ -116,7 +116,6 @@ struct AttentionArgs {
     float scale;          // of the scores, times log2 e
     uint32_t group, splits, tiles;
     uint32_t chunk, tile;   // 64-position steps of a split, rows of a tile
-    int vector_q;         // rows of q on 16-byte boundaries
 };
 
 // Steps of each split of a row tile that sees `steps`: the planned number, or more
@@ -131,24 +130,16 @@ __device__ __forceinline__ int32_t split_chunk(const AttentionArgs& a, int32_t s
 // that the row's largest lies in [2^14, 2^15), in planes; cs takes a score in units
 // of that back (times log2 e), qs is the row's sum in them.
 template <int D>
-__device__ __forceinline__ void load_query(const float* q, bool vector, uint32_t g, float scale,
+__device__ __forceinline__ void load_query(const float* q, uint32_t g, float scale,
     f16x8 (&hi)[D / 32], f16x8 (&lo)[D / 32], float& cs, float& qs)
 {
     float v[D / 4];
     q += 8 * g;
 #pragma unroll
     for (int j = 0; j < D / 32; j++) {
-        if (vector) {
-            const float4 x = *reinterpret_cast<const float4*>(q + 32 * j);
-            const float4 y = *reinterpret_cast<const float4*>(q + 32 * j + 4);
-            v[8 * j] = x.x, v[8 * j + 1] = x.y, v[8 * j + 2] = x.z, v[8 * j + 3] = x.w;
-            v[8 * j + 4] = y.x, v[8 * j + 5] = y.y, v[8 * j + 6] = y.z, v[8 * j + 7] = y.w;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                v[8 * j + e] = q[32 * j + e];
-            }
-        }
+        const float4 x = load4(q + 32 * j), y = load4(q + 32 * j + 4);
+        v[8 * j] = x.x, v[8 * j + 1] = x.y, v[8 * j + 2] = x.z, v[8 * j + 3] = x.w;
+        v[8 * j + 4] = y.x, v[8 * j + 5] = y.y, v[8 * j + 6] = y.z, v[8 * j + 7] = y.w;
     }
     float most = 0, sum = 0;
 #pragma unroll
@@ -415,7 +406,7 @@ k_paged_attention(AttentionArgs a)
             c.limit[n] = last < 0 ? -1 : (int32_t)(last < capacity ? last : capacity - 1);
             const float* q = a.q + (size_t)(span.begin + t) * a.q_stride +
                 ((size_t)h * a.group + row % a.group) * D;
-            load_query<D>(q, a.vector_q, g, a.scale, c.hi[n], c.lo[n], c.cs[n], c.qs[n]);
+            load_query<D>(q, g, a.scale, c.hi[n], c.lo[n], c.cs[n], c.qs[n]);
             c.m[n] = -__builtin_inff();
             c.sum[n] = c.offset[n] = 0;
 #pragma unroll
@@ -877,7 +868,7 @@ k_paged_decode(AttentionArgs a)
             ((size_t)h * a.group + row % a.group) * D;
         if constexpr (Decode<D, Q4, C>::SHARED) {
             f16x8 hi[D / 32], lo[D / 32];
-            load_query<D>(q, a.vector_q, c.g, a.scale, hi, lo, c.cs, c.qs);
+            load_query<D>(q, c.g, a.scale, hi, lo, c.cs, c.qs);
             __syncthreads();   // the previous tile's readers
             if (wave == 0) {
 #pragma unroll
@@ -888,7 +879,7 @@ k_paged_decode(AttentionArgs a)
             }
             __syncthreads();
         } else {
-            load_query<D>(q, a.vector_q, c.g, a.scale, c.hi, c.lo, c.cs, c.qs);
+            load_query<D>(q, c.g, a.scale, c.hi, c.lo, c.cs, c.qs);
         }
         int32_t turn = 0;
         if constexpr (Q4) {
@@ -1159,7 +1150,7 @@ extern "C" int lh_launch_paged_attention(const lh_paged_cache* cache, const lh_p
     const AttentionArgs a = {pages_of(cache), batch_of(batch), q, out, part, tops, q_stride,
         out_stride,
         (((uint64_t)1 << 32) + in_page - 1) / in_page, scale * 1.44269504088896341f, group,
-        p.splits, p.tiles, p.chunk, p.tile, ((uintptr_t)q & 15) == 0 && q_stride % 4 == 0};
+        p.splits, p.tiles, p.chunk, p.tile};
     LH_FOR_CACHE(cache, attention, cache, batch, p, a, s);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
