@@ -8,7 +8,7 @@
 // operand of a 16x16x32 matrix instruction. Then the scales: a tile's hold for g
 // and group j the four BF16 scales of rows 4 g .. 4 g + 3, the rows of a lane's
 // results. Rows and columns past the matrix have code 8 and scale 0.
-#include "lh_device.h"
+#include "lh_nibbles.h"
 #include "lh_serving.h"
 
 namespace lh {
@@ -106,37 +106,363 @@ k_q4_quantize(const float* __restrict__ w, Q4Shape p, uint8_t* __restrict__ pack
     reinterpret_cast<uint32_t*>(packed)[((size_t)tile * p.blocks + block) * 256 + i] = word;
 }
 
-// One wave a row and token, one packed word a lane at a time.
-__global__ void __launch_bounds__(256)
-k_q4_rows(const uint8_t* __restrict__ packed, Q4Shape p, const float* __restrict__ x,
-    size_t x_stride, float* __restrict__ y, size_t y_stride)
+// The product. A wave takes 128-column blocks of RT row tiles for NT tiles of 16
+// tokens: y^T tile [16 rows][16 tokens] = W X^T by 16x16x32 FP16 matrix instructions,
+// W the codes minus 8 (exact), X two planes h + l of x times a power of two. A
+// group's sums are formed from 0 and join the row's by its scale in FP32, so a scale
+// never rounds a weight. Eight waves split the columns and meet in LDS. Codes and
+// scales of the next block are on their way while one is multiplied.
+enum { WAVES = 8 };
+
+struct Q4Args {
+    const uint8_t* packed;
+    Q4Shape p;
+    const float* x;
+    float* y;
+    size_t x_stride, y_stride;
+    uint32_t tokens, per;       // per: blocks of a wave
+    const f16x8* planes;        // [token tile][block][32-column step][plane][lane]
+    const float* factors;       // [token]: the power of two back
+    float* part;                // [split][token][16 tiles] where blockIdx.z splits
+};
+
+// A block's codes and scales of RT tiles. PER: scales of a row in a block.
+template <int PER, int RT>
+struct Q4Block {
+    u32x4 w[RT];
+    uint32_t s[RT][2 * PER];   // BF16 pairs: group j's rows 4 g .. + 3 in words 2 j, 2 j + 1
+
+    __device__ __forceinline__ void load(const Q4Args& a, uint32_t tile, uint32_t block,
+        uint32_t lane)
+    {
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            // Tiles past the last repeat it and are not stored.
+            const uint32_t mine = tile + t < a.p.tiles ? tile + t : a.p.tiles - 1;
+            const size_t at = (size_t)mine * a.p.blocks + block;
+            w[t] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(a.packed) +
+                at * 64 + lane);
+            const uint32_t* scale = reinterpret_cast<const uint32_t*>(a.packed +
+                q4_scales_at(a.p) + at * (32 * PER)) + (lane >> 4) * (2 * PER);
+#pragma unroll
+            for (int i = 0; i < 2 * PER; i++) {
+                s[t][i] = scale[i];
+            }
+        }
+    }
+};
+
+template <int PER, int RT, int NT>
+__device__ __forceinline__ void q4_multiply(const Q4Block<PER, RT>& b, const f16x8 (&x)[NT][4][2],
+    floatx4 (&acc)[RT][NT], const NibbleMasks& mask)
 {
-    const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const size_t token = blockIdx.y;
-    if (row >= p.rows) {
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        floatx4 d[NT];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const f16x8 w = codes_minus8(b.w[t][j], mask);
+            constexpr int STEPS = 4 / PER;   // 32-column steps of a group
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                if (j % STEPS == 0) {
+                    d[n] = (floatx4){0, 0, 0, 0};
+                }
+                d[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, x[n][j][0], d[n], 0, 0, 0);
+                d[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, x[n][j][1], d[n], 0, 0, 0);
+            }
+            if (j % STEPS == STEPS - 1) {
+                const uint32_t low = b.s[t][2 * (j / STEPS)], high = b.s[t][2 * (j / STEPS) + 1];
+                const float s[4] = {bf16_to_f32(low & 0xffffu),
+                    __uint_as_float(low & 0xffff0000u), bf16_to_f32(high & 0xffffu),
+                    __uint_as_float(high & 0xffff0000u)};
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        acc[t][n][i] = __builtin_fmaf(s[i], d[n][i], acc[t][n][i]);
+                    }
+                }
+            }
+        }
+    }
+}
+
+// The eight waves' sums of RT x NT tiles (each times its factor) to y, or to the
+// split's part.
+template <int RT, int NT>
+__device__ __forceinline__ void q4_store(const Q4Args& a, floatx4* joined,
+    const floatx4 (&acc)[RT][NT], const float (&factor)[NT], uint32_t tile, uint32_t token0)
+{
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            floatx4 v = acc[t][n];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                v[i] *= factor[n];
+            }
+            joined[((t * NT + n) * WAVES + wave) * 64 + lane] = v;
+        }
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < RT * NT * 64; i += 64 * WAVES) {
+        const uint32_t l = i & 63, which = i >> 6, t = which / NT, n = which % NT;
+        floatx4 v = joined[which * WAVES * 64 + l];
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) {
+            const floatx4 o = joined[(which * WAVES + w) * 64 + l];
+            v += o;
+        }
+        const uint32_t token = token0 + 16 * n + (l & 15), row = (tile + t) * 16 + 4 * (l >> 4);
+        if (token >= a.tokens || tile + t >= a.p.tiles) {
+            continue;
+        }
+        if (gridDim.z > 1) {
+            const size_t width = (size_t)a.p.tiles * 16;
+            *reinterpret_cast<floatx4*>(a.part + ((size_t)blockIdx.z * a.tokens + token) * width +
+                row) = v;
+            continue;
+        }
+        float* y = a.y + token * a.y_stride + row;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (row + e < a.p.rows) {
+                y[e] = v[e];
+            }
+        }
+    }
+}
+
+// Few tokens: every wave turns its own columns of x into planes in LDS first (its own
+// power of two for each token), with the first block's codes on their way. At most
+// STAGED (token, block) pairs a wave; no scratch and one launch.
+enum { STAGED = 16 };
+
+template <int PER, int RT>
+__global__ void __launch_bounds__(64 * WAVES)
+k_q4_few(Q4Args a)
+{
+    __shared__ union {
+        f16x8 planes[WAVES][STAGED * 32];          // [block][step][plane][g][token]
+        floatx4 joined[RT * WAVES * 64];
+    } u;
+    __shared__ uint32_t most[WAVES][16];
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t tile = blockIdx.x * RT, tokens = a.tokens;
+    const uint32_t first = wave * a.per;
+    const uint32_t end = first + a.per < a.p.blocks ? first + a.per : a.p.blocks;
+    // Chunks of eight columns: lane l takes chunks l, l + 64 .. of (token, chunk).
+    constexpr int EACH = STAGED / 4;
+    const uint32_t width = a.per * 16;
+    const float inverse = 1.0f / (float)width;
+    float v[EACH][8];
+    uint32_t token[EACH], chunk[EACH];
+    if (lane < 16) {
+        most[wave][lane] = 0;
+    }
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+        const uint32_t id = 64 * i + lane;
+        token[i] = (uint32_t)(((float)id + 0.5f) * inverse);   // exact: ids are below 2^10
+        chunk[i] = id - token[i] * width;
+        const uint32_t col = first * 128 + chunk[i] * 8;
+        if (token[i] < tokens && col < a.p.cols) {
+            const float* x = a.x + token[i] * a.x_stride + col;
+            const float4 p = load4(x), q = load4(x + 4);
+            v[i][0] = p.x, v[i][1] = p.y, v[i][2] = p.z, v[i][3] = p.w;
+            v[i][4] = q.x, v[i][5] = q.y, v[i][6] = q.z, v[i][7] = q.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                v[i][e] = 0;
+            }
+        }
+    }
+    Q4Block<PER, RT> now;
+    if (first < end) {
+        now.load(a, tile, first, lane);
+    }
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+        uint32_t m = 0;   // magnitudes order as their bits; an Inf or NaN is the largest
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const uint32_t bits = __float_as_uint(v[i][e]) & 0x7fffffffu;
+            m = m > bits ? m : bits;
+        }
+        if (token[i] < tokens) {
+            atomicMax(&most[wave][token[i]], m);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+        if (token[i] < tokens) {
+            const float up = exp2i(row_exponent(__uint_as_float(most[wave][token[i]])));
+            float s[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                s[e] = v[i][e] * up;
+            }
+            f16x8 hi, lo;
+            planes8(s, hi, lo);
+            // Chunk: block, step j and g in turn.
+            f16x8* to = u.planes[wave] + ((chunk[i] >> 2) * 8 + (chunk[i] & 3)) * tokens + token[i];
+            to[0] = hi;
+            to[4 * tokens] = lo;
+        }
+    }
+    __syncthreads();
+    const NibbleMasks mask;
+    const uint32_t mine = (lane & 15) < tokens ? lane & 15 : tokens - 1;
+    float factor[1] = {exp2i(-row_exponent(__uint_as_float(most[wave][mine])))};
+    floatx4 acc[RT][1];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        acc[t][0] = (floatx4){0, 0, 0, 0};
+    }
+    for (uint32_t b = first; b < end; b++) {
+        Q4Block<PER, RT> next = now;
+        if (b + 1 < end) {
+            next.load(a, tile, b + 1, lane);
+        }
+        f16x8 x[1][4][2];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+#pragma unroll
+            for (int plane = 0; plane < 2; plane++) {
+                x[0][j][plane] = u.planes[wave][(((b - first) * 4 + j) * 8 + plane * 4 + g) *
+                    tokens + mine];
+            }
+        }
+        q4_multiply<PER, RT, 1>(now, x, acc, mask);
+        now = next;
+    }
+    __syncthreads();   // the planes are done with
+    q4_store<RT, 1>(a, u.joined, acc, factor, tile, 0);
+}
+
+// More tokens: planes made once, by one workgroup a token.
+__global__ void __launch_bounds__(256)
+k_q4_planes(Q4Args a, f16x8* planes, float* factors)
+{
+    __shared__ uint32_t most[4];
+    const uint32_t token = blockIdx.x;
+    const float* x = a.x + token * a.x_stride;
+    uint32_t m = 0;
+    for (uint32_t c = threadIdx.x * 4; c < a.p.cols; c += 1024) {
+        const float4 v = load4(x + c);
+        const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint32_t bits = __float_as_uint(f[e]) & 0x7fffffffu;
+            m = m > bits ? m : bits;
+        }
+    }
+    for (int s = 32; s; s >>= 1) {
+        const uint32_t o = __shfl_xor(m, s);
+        m = m > o ? m : o;
+    }
+    if ((threadIdx.x & 63) == 0) {
+        most[threadIdx.x >> 6] = m;
+    }
+    __syncthreads();
+    for (int w = 0; w < 4; w++) {
+        m = m > most[w] ? m : most[w];
+    }
+    const int e2 = row_exponent(__uint_as_float(m));
+    const float up = exp2i(e2);
+    if (threadIdx.x == 0) {
+        factors[token] = exp2i(-e2);
+    }
+    for (uint32_t c = threadIdx.x * 8; c < a.p.blocks * 128; c += 2048) {
+        float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (c < a.p.cols) {
+            const float4 p = load4(x + c), q = load4(x + c + 4);
+            s[0] = p.x * up, s[1] = p.y * up, s[2] = p.z * up, s[3] = p.w * up;
+            s[4] = q.x * up, s[5] = q.y * up, s[6] = q.z * up, s[7] = q.w * up;
+        }
+        f16x8 hi, lo;
+        planes8(s, hi, lo);
+        const uint32_t block = c >> 7, j = (c >> 5) & 3, g = (c >> 3) & 3;
+        f16x8* to = planes + ((((size_t)(token >> 4) * a.p.blocks + block) * 4 + j) * 2) * 64 +
+            16 * g + (token & 15);
+        to[0] = hi;
+        to[64] = lo;
+    }
+}
+
+// grid (row tiles / RT, token tiles / NT, column splits). Planes of tokens past the last
+// hold anything: a column's sums are its own and these are not stored.
+template <int PER, int RT, int NT>
+__global__ void __launch_bounds__(64 * WAVES)
+k_q4_many(Q4Args a)
+{
+    __shared__ floatx4 joined[RT * NT * WAVES * 64];
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t tile = blockIdx.x * RT, token0 = blockIdx.y * NT * 16;
+    const uint32_t first = (blockIdx.z * WAVES + wave) * a.per;
+    const uint32_t end = first + a.per < a.p.blocks ? first + a.per : a.p.blocks;
+    const uint32_t last = (a.tokens - 1) >> 4;
+    const f16x8* planes[NT];
+    float factor[NT];
+    floatx4 acc[RT][NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const uint32_t at = blockIdx.y * NT + n < last ? blockIdx.y * NT + n : last;
+        planes[n] = a.planes + (size_t)at * a.p.blocks * 512 + lane;
+        const uint32_t token = 16 * at + (lane & 15);
+        factor[n] = a.factors[token < a.tokens ? token : a.tokens - 1];
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            acc[t][n] = (floatx4){0, 0, 0, 0};
+        }
+    }
+    const NibbleMasks mask;
+    Q4Block<PER, RT> now;
+    if (first < end) {
+        now.load(a, tile, first, lane);
+    }
+    for (uint32_t b = first; b < end; b++) {
+        Q4Block<PER, RT> next = now;
+        if (b + 1 < end) {
+            next.load(a, tile, b + 1, lane);
+        }
+        f16x8 x[NT][4][2];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                x[n][j][0] = planes[n][((size_t)b * 4 + j) * 128];
+                x[n][j][1] = planes[n][((size_t)b * 4 + j) * 128 + 64];
+            }
+        }
+        q4_multiply<PER, RT, NT>(now, x, acc, mask);
+        now = next;
+    }
+    q4_store<RT, NT>(a, joined, acc, factor, tile, token0);
+}
+
+// y = the sum of the column splits' parts, in their order.
+__global__ void __launch_bounds__(256)
+k_q4_join(Q4Args a, uint32_t splits)
+{
+    const uint32_t row = blockIdx.x * 256 + threadIdx.x, token = blockIdx.y;
+    if (row >= a.p.rows) {
         return;
     }
-    const uint32_t tile = row >> 4, r = row & 15;
-    float sum = 0;
-    for (uint32_t col = lane * 8; col < p.cols; col += 512) {
-        const uint32_t block = col >> 7, j = (col >> 5) & 3, g = (col >> 3) & 3;
-        const uint32_t word = reinterpret_cast<const uint32_t*>(packed)
-            [((size_t)tile * p.blocks + block) * 256 + (g * 16 + r) * 4 + j];
-        const float s = bf16_to_f32(*reinterpret_cast<const uint16_t*>(
-            packed + q4_scale_at(p, tile, block, r, (col & 127) / p.group)));
-        float part = 0;
-        for (uint32_t e = 0; e < 8; e++) {
-            const int code = (word >> (4 * (e >> 1) + 16 * (e & 1))) & 15;
-            const float v = x[token * x_stride + col + e];
-            part = __builtin_fmaf((float)(code - 8), v, part);
-            part = __builtin_fmaf(0.0f, v, part);   // an Inf is a NaN for the whole row
-        }
-        sum = __builtin_fmaf(s, part, sum);
+    const size_t width = (size_t)a.p.tiles * 16, step = width * a.tokens;
+    const float* part = a.part + token * width + row;
+    float v = part[0];
+    for (uint32_t i = 1; i < splits; i++) {
+        v += part[i * step];
     }
-    sum = wave_tree64(sum);
-    if (lane == 0) {
-        y[token * y_stride + row] = sum;
-    }
+    a.y[token * a.y_stride + row] = v;
 }
 
 }  // namespace lh
@@ -160,20 +486,116 @@ extern "C" int lh_launch_q4_quantize(const float* w, uint32_t rows, uint32_t col
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
+// How a product runs. few: planes in the kernel itself. Otherwise nt token tiles a
+// workgroup and `splits` column splits, with scratch for planes, factors and parts.
+struct Q4Plan {
+    bool few;
+    uint32_t nt, rt, splits, per;
+    size_t planes, factors;   // bytes
+};
+
+static Q4Plan q4_plan(uint32_t rows, uint32_t cols, uint32_t tokens)
+{
+    const uint32_t blocks = (cols + 127) / 128, tiles = (rows + 15) / 16;
+    Q4Plan p = {};
+    p.per = (blocks + WAVES - 1) / WAVES;
+    p.splits = 1;
+    p.few = tokens <= 16 && tokens * p.per <= STAGED;
+    // Row tiles of a workgroup: more save reads of x, as long as the chip is full.
+    p.rt = tiles >= 1024 ? 4 : tiles >= 512 ? 2 : 1;
+    if (p.few) {
+        return p;
+    }
+    const uint32_t tt = (tokens + 15) / 16;
+    p.nt = tt < 4 ? tt : 4;
+    p.rt = tiles >= 512 && p.nt <= 2 ? 4 : 2;   // registers for RT * NT <= 8 tiles
+    const uint32_t groups = (tiles + p.rt - 1) / p.rt * ((tt + p.nt - 1) / p.nt);
+    uint32_t splits = (256 + groups - 1) / groups;
+    const uint32_t most = (blocks + 2 * WAVES - 1) / (2 * WAVES);   // two blocks a wave
+    splits = splits < most ? splits : most;
+    p.per = (blocks + splits * WAVES - 1) / (splits * WAVES);
+    p.splits = (blocks + p.per * WAVES - 1) / (p.per * WAVES);
+    p.planes = (size_t)tt * blocks * 8192;
+    p.factors = lh_round16((size_t)tokens * 4);
+    return p;
+}
+
+template <int PER>
+static void q4_few(const Q4Plan& p, const Q4Args& a, hipStream_t s)
+{
+    const dim3 grid((a.p.tiles + p.rt - 1) / p.rt), block(64 * WAVES);
+    switch (p.rt) {
+    case 1: hipLaunchKernelGGL((k_q4_few<PER, 1>), grid, block, 0, s, a); break;
+    case 2: hipLaunchKernelGGL((k_q4_few<PER, 2>), grid, block, 0, s, a); break;
+    default: hipLaunchKernelGGL((k_q4_few<PER, 4>), grid, block, 0, s, a); break;
+    }
+}
+
+template <int PER>
+static void q4_many(const Q4Plan& p, const Q4Args& a, hipStream_t s)
+{
+    const uint32_t tt = (a.tokens + 15) / 16;
+    const dim3 grid((a.p.tiles + p.rt - 1) / p.rt, (tt + p.nt - 1) / p.nt, p.splits);
+    const dim3 block(64 * WAVES);
+    switch (p.nt * 8 + p.rt) {
+    case 8 + 2: hipLaunchKernelGGL((k_q4_many<PER, 2, 1>), grid, block, 0, s, a); break;
+    case 8 + 4: hipLaunchKernelGGL((k_q4_many<PER, 4, 1>), grid, block, 0, s, a); break;
+    case 16 + 2: hipLaunchKernelGGL((k_q4_many<PER, 2, 2>), grid, block, 0, s, a); break;
+    case 16 + 4: hipLaunchKernelGGL((k_q4_many<PER, 4, 2>), grid, block, 0, s, a); break;
+    case 24 + 2: hipLaunchKernelGGL((k_q4_many<PER, 2, 3>), grid, block, 0, s, a); break;
+    default: hipLaunchKernelGGL((k_q4_many<PER, 2, 4>), grid, block, 0, s, a); break;
+    }
+}
+
+template <int PER>
+static void q4_product(const Q4Plan& p, const Q4Args& a, hipStream_t s)
+{
+    if (p.few) {
+        q4_few<PER>(p, a, s);
+    } else {
+        q4_many<PER>(p, a, s);
+    }
+}
+
+// For any number of rows: splits appear below 256 workgroups and bring them to less
+// than 512, of at most four row tiles and (past 64 tokens more workgroups, not more
+// tokens) 64 tokens, so their parts hold at most 512 * 4 * 16 rows of min(tokens, 64).
 extern "C" size_t lh_q4_scratch_bytes(uint32_t cols, uint32_t tokens)
 {
-    (void)cols;
-    (void)tokens;
-    return 0;
+    const Q4Plan p = q4_plan(1, cols, tokens);
+    if (p.few) {
+        return 0;
+    }
+    const size_t parts = cols > 128 * 2 * WAVES ? (size_t)512 * 4 * 16 * 4 : 0;
+    return p.planes + p.factors + parts * (tokens < 64 ? tokens : 64);
 }
 
 extern "C" int lh_launch_q4_matvec(const uint8_t* packed, const float* x, size_t x_stride,
     float* y, size_t y_stride, uint32_t rows, uint32_t cols, uint32_t group, uint32_t tokens,
     uint8_t* scratch, hipStream_t s)
 {
-    (void)scratch;
-    const Q4Shape p = q4_shape(rows, cols, group);
-    hipLaunchKernelGGL(k_q4_rows, dim3((rows + 3) / 4, tokens), dim3(256), 0, s, packed, p, x,
-        x_stride, y, y_stride);
+    const Q4Plan p = q4_plan(rows, cols, tokens);
+    f16x8* planes = reinterpret_cast<f16x8*>(scratch);
+    float* factors = reinterpret_cast<float*>(scratch + p.planes);
+    const Q4Args a = {packed, q4_shape(rows, cols, group), x, y, x_stride, y_stride, tokens, p.per,
+        planes, factors, reinterpret_cast<float*>(scratch + p.planes + p.factors)};
+    if (!p.few) {
+        hipLaunchKernelGGL(k_q4_planes, dim3(tokens), dim3(256), 0, s, a, planes, factors);
+        if (hipGetLastError() != hipSuccess) {
+            return -1;
+        }
+    }
+    switch (group) {
+    case 32: q4_product<4>(p, a, s); break;
+    case 64: q4_product<2>(p, a, s); break;
+    default: q4_product<1>(p, a, s); break;
+    }
+    if (hipGetLastError() != hipSuccess) {
+        return -1;
+    }
+    if (p.splits > 1) {
+        hipLaunchKernelGGL(k_q4_join, dim3((rows + 255) / 256, tokens), dim3(256), 0, s, a,
+            p.splits);
+    }
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
