@@ -188,42 +188,31 @@ __device__ __forceinline__ void q4_multiply(const Q4Block<PER, RT>& b, const f16
     }
 }
 
-// The eight waves' sums of RT x NT tiles (each times its factor) to y, or to the
-// split's part.
-template <int RT, int NT>
+// The eight waves' sums of RT tiles (each times its factor) to y.
+template <int RT>
 __device__ __forceinline__ void q4_store(const Q4Args& a, floatx4* joined,
-    const floatx4 (&acc)[RT][NT], const float (&factor)[NT], uint32_t tile, uint32_t token0)
+    const floatx4 (&acc)[RT][1], float factor, uint32_t tile)
 {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int t = 0; t < RT; t++) {
+        floatx4 v = acc[t][0];
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            floatx4 v = acc[t][n];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                v[i] *= factor[n];
-            }
-            joined[((t * NT + n) * WAVES + wave) * 64 + lane] = v;
+        for (int i = 0; i < 4; i++) {
+            v[i] *= factor;
         }
+        joined[(t * WAVES + wave) * 64 + lane] = v;
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < RT * NT * 64; i += 64 * WAVES) {
-        const uint32_t l = i & 63, which = i >> 6, t = which / NT, n = which % NT;
-        floatx4 v = joined[which * WAVES * 64 + l];
+    for (uint32_t i = threadIdx.x; i < RT * 64; i += 64 * WAVES) {
+        const uint32_t l = i & 63, t = i >> 6;
+        floatx4 v = joined[t * WAVES * 64 + l];
 #pragma unroll
         for (int w = 1; w < WAVES; w++) {
-            const floatx4 o = joined[(which * WAVES + w) * 64 + l];
-            v += o;
+            v += joined[(t * WAVES + w) * 64 + l];
         }
-        const uint32_t token = token0 + 16 * n + (l & 15), row = (tile + t) * 16 + 4 * (l >> 4);
-        if (token >= a.tokens || tile + t >= a.p.tiles) {
-            continue;
-        }
-        if (gridDim.z > 1) {
-            const size_t width = (size_t)a.p.tiles * 16;
-            *reinterpret_cast<floatx4*>(a.part + ((size_t)blockIdx.z * a.tokens + token) * width +
-                row) = v;
+        const uint32_t token = l & 15, row = (tile + t) * 16 + 4 * (l >> 4);
+        if (token >= a.tokens) {
             continue;
         }
         float* y = a.y + token * a.y_stride + row;
@@ -238,26 +227,32 @@ __device__ __forceinline__ void q4_store(const Q4Args& a, floatx4* joined,
 
 // Few tokens: every wave turns its own columns of x into planes in LDS first (its own
 // power of two for each token), with the first block's codes on their way. At most
-// STAGED (token, block) pairs a wave; no scratch and one launch.
-enum { STAGED = 16 };
+// STAGED (token, block) pairs a wave, 512 bytes each; no scratch and one launch.
+enum { STAGED = 32 };
+
+// LDS: the planes, then the waves' sums.
+static size_t q4_few_lds(uint32_t tokens, uint32_t per, uint32_t rt)
+{
+    const size_t planes = (size_t)WAVES * tokens * per * 512, sums = (size_t)rt * WAVES * 1024;
+    return planes > sums ? planes : sums;
+}
 
 template <int PER, int RT>
 __global__ void __launch_bounds__(64 * WAVES)
 k_q4_few(Q4Args a)
 {
-    __shared__ union {
-        f16x8 planes[WAVES][STAGED * 32];          // [block][step][plane][g][token]
-        floatx4 joined[RT * WAVES * 64];
-    } u;
+    extern __shared__ floatx4 shared[];
     __shared__ uint32_t most[WAVES][16];
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t tile = blockIdx.x * RT, tokens = a.tokens;
     const uint32_t first = wave * a.per;
+    // [block][step][plane][g][token]
+    f16x8* planes = reinterpret_cast<f16x8*>(shared) + wave * tokens * a.per * 32;
     const uint32_t end = first + a.per < a.p.blocks ? first + a.per : a.p.blocks;
     // Chunks of eight columns: lane l takes chunks l, l + 64 .. of (token, chunk).
     constexpr int EACH = STAGED / 4;
-    const uint32_t width = a.per * 16;
+    const uint32_t width = a.per * 16, used = tokens * width;
     const float inverse = 1.0f / (float)width;
     float v[EACH][8];
     uint32_t token[EACH], chunk[EACH];
@@ -266,6 +261,9 @@ k_q4_few(Q4Args a)
     }
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
+        if (64u * i >= used) {
+            break;
+        }
         const uint32_t id = 64 * i + lane;
         token[i] = (uint32_t)(((float)id + 0.5f) * inverse);   // exact: ids are below 2^10
         chunk[i] = id - token[i] * width;
@@ -288,6 +286,9 @@ k_q4_few(Q4Args a)
     }
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
+        if (64u * i >= used) {
+            break;
+        }
         uint32_t m = 0;   // magnitudes order as their bits; an Inf or NaN is the largest
 #pragma unroll
         for (int e = 0; e < 8; e++) {
@@ -301,6 +302,9 @@ k_q4_few(Q4Args a)
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
+        if (64u * i >= used) {
+            break;
+        }
         if (token[i] < tokens) {
             const float up = exp2i(row_exponent(__uint_as_float(most[wave][token[i]])));
             float s[8];
@@ -311,7 +315,7 @@ k_q4_few(Q4Args a)
             f16x8 hi, lo;
             planes8(s, hi, lo);
             // Chunk: block, step j and g in turn.
-            f16x8* to = u.planes[wave] + ((chunk[i] >> 2) * 8 + (chunk[i] & 3)) * tokens + token[i];
+            f16x8* to = planes + ((chunk[i] >> 2) * 8 + (chunk[i] & 3)) * tokens + token[i];
             to[0] = hi;
             to[4 * tokens] = lo;
         }
@@ -335,33 +339,54 @@ k_q4_few(Q4Args a)
         for (int j = 0; j < 4; j++) {
 #pragma unroll
             for (int plane = 0; plane < 2; plane++) {
-                x[0][j][plane] = u.planes[wave][(((b - first) * 4 + j) * 8 + plane * 4 + g) *
-                    tokens + mine];
+                x[0][j][plane] = planes[(((b - first) * 4 + j) * 8 + plane * 4 + g) * tokens +
+                    mine];
             }
         }
         q4_multiply<PER, RT, 1>(now, x, acc, mask);
         now = next;
     }
     __syncthreads();   // the planes are done with
-    q4_store<RT, 1>(a, u.joined, acc, factor, tile, 0);
+    q4_store<RT>(a, shared, acc, factor[0], tile);
 }
 
-// More tokens: planes made once, by one workgroup a token.
-__global__ void __launch_bounds__(256)
+// More tokens: planes made once, by one workgroup a token. A thread holds its first
+// two chunks of eight columns (all of them up to 16384 columns) between the two passes.
+__global__ void __launch_bounds__(1024)
 k_q4_planes(Q4Args a, f16x8* planes, float* factors)
 {
-    __shared__ uint32_t most[4];
-    const uint32_t token = blockIdx.x;
+    __shared__ uint32_t most[16];
+    const uint32_t token = blockIdx.x, chunks = a.p.blocks * 16;
     const float* x = a.x + token * a.x_stride;
-    uint32_t m = 0;
-    for (uint32_t c = threadIdx.x * 4; c < a.p.cols; c += 1024) {
-        const float4 v = load4(x + c);
-        const float f[4] = {v.x, v.y, v.z, v.w};
+    auto load = [&](uint32_t chunk, float (&v)[8]) __attribute__((always_inline)) {
+        if (chunk * 8 < a.p.cols) {
+            const float4 p = load4(x + chunk * 8), q = load4(x + chunk * 8 + 4);
+            v[0] = p.x, v[1] = p.y, v[2] = p.z, v[3] = p.w;
+            v[4] = q.x, v[5] = q.y, v[6] = q.z, v[7] = q.w;
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const uint32_t bits = __float_as_uint(f[e]) & 0x7fffffffu;
+            for (int e = 0; e < 8; e++) {
+                v[e] = 0;
+            }
+        }
+    };
+    uint32_t m = 0;
+    auto largest = [&](const float (&v)[8]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const uint32_t bits = __float_as_uint(v[e]) & 0x7fffffffu;
             m = m > bits ? m : bits;
         }
+    };
+    float v0[8], v1[8];
+    load(threadIdx.x, v0);
+    load(threadIdx.x + 1024, v1);
+    largest(v0);
+    largest(v1);
+    for (uint32_t c = threadIdx.x + 2048; c < chunks; c += 1024) {
+        float v[8];
+        load(c, v);
+        largest(v);
     }
     for (int s = 32; s; s >>= 1) {
         const uint32_t o = __shfl_xor(m, s);
@@ -371,7 +396,7 @@ k_q4_planes(Q4Args a, f16x8* planes, float* factors)
         most[threadIdx.x >> 6] = m;
     }
     __syncthreads();
-    for (int w = 0; w < 4; w++) {
+    for (int w = 0; w < 16; w++) {
         m = m > most[w] ? m : most[w];
     }
     const int e2 = row_exponent(__uint_as_float(m));
@@ -379,73 +404,124 @@ k_q4_planes(Q4Args a, f16x8* planes, float* factors)
     if (threadIdx.x == 0) {
         factors[token] = exp2i(-e2);
     }
-    for (uint32_t c = threadIdx.x * 8; c < a.p.blocks * 128; c += 2048) {
-        float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (c < a.p.cols) {
-            const float4 p = load4(x + c), q = load4(x + c + 4);
-            s[0] = p.x * up, s[1] = p.y * up, s[2] = p.z * up, s[3] = p.w * up;
-            s[4] = q.x * up, s[5] = q.y * up, s[6] = q.z * up, s[7] = q.w * up;
+    auto store = [&](uint32_t c, const float (&v)[8]) __attribute__((always_inline)) {
+        if (c >= chunks) {
+            return;
+        }
+        float s[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            s[e] = v[e] * up;
         }
         f16x8 hi, lo;
         planes8(s, hi, lo);
-        const uint32_t block = c >> 7, j = (c >> 5) & 3, g = (c >> 3) & 3;
-        f16x8* to = planes + ((((size_t)(token >> 4) * a.p.blocks + block) * 4 + j) * 2) * 64 +
-            16 * g + (token & 15);
+        f16x8* to = planes + ((size_t)(token >> 4) * a.p.blocks * 8 + (c >> 2) * 2) * 64 +
+            16 * (c & 3) + (token & 15);
         to[0] = hi;
         to[64] = lo;
+    };
+    store(threadIdx.x, v0);
+    store(threadIdx.x + 1024, v1);
+    for (uint32_t c = threadIdx.x + 2048; c < chunks; c += 1024) {
+        float v[8];
+        load(c, v);
+        store(c, v);
     }
 }
 
-// grid (row tiles / RT, token tiles / NT, column splits). Planes of tokens past the last
-// hold anything: a column's sums are its own and these are not stored.
-template <int PER, int RT, int NT>
-__global__ void __launch_bounds__(64 * WAVES)
+// Four waves with two row tiles each share the planes of NT token tiles in LDS, which
+// is filled a block ahead by loads straight into it; codes come a block ahead too.
+// grid (8-tile row groups, token tiles / NT, column splits). Planes of tokens past the
+// last hold anything: a column's sums are its own and these are not stored.
+template <int PER, int NT>
+__global__ void __launch_bounds__(256)
 k_q4_many(Q4Args a)
 {
-    __shared__ floatx4 joined[RT * NT * WAVES * 64];
-    const uint32_t lane = threadIdx.x & 63;
+    constexpr int RT = 2, BLOCK = NT * 512;   // f16x8 of a block's planes
+    __shared__ f16x8 shared[2][BLOCK];
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t tile = blockIdx.x * RT, token0 = blockIdx.y * NT * 16;
-    const uint32_t first = (blockIdx.z * WAVES + wave) * a.per;
+    const uint32_t tile = (blockIdx.x * 4 + wave) * RT, tile0 = blockIdx.y * NT;
+    const uint32_t first = blockIdx.z * a.per;
     const uint32_t end = first + a.per < a.p.blocks ? first + a.per : a.p.blocks;
     const uint32_t last = (a.tokens - 1) >> 4;
-    const f16x8* planes[NT];
-    float factor[NT];
+    auto stage = [&](uint32_t block, f16x8* to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 2 * NT; i++) {
+            // 256 f16x8: half a token tile's block; a wave writes 1 KiB in lane order.
+            const uint32_t n = i / 2, at = tile0 + n < last ? tile0 + n : last;
+            const f16x8* from = a.planes + ((size_t)at * a.p.blocks + block) * 512 +
+                (i & 1) * 256 + threadIdx.x;
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void*)from,
+                (__attribute__((address_space(3))) void*)(to + i * 256 + wave * 64), 16, 0, 0);
+        }
+    };
     floatx4 acc[RT][NT];
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        const uint32_t at = blockIdx.y * NT + n < last ? blockIdx.y * NT + n : last;
-        planes[n] = a.planes + (size_t)at * a.p.blocks * 512 + lane;
-        const uint32_t token = 16 * at + (lane & 15);
-        factor[n] = a.factors[token < a.tokens ? token : a.tokens - 1];
+    for (int t = 0; t < RT; t++) {
 #pragma unroll
-        for (int t = 0; t < RT; t++) {
+        for (int n = 0; n < NT; n++) {
             acc[t][n] = (floatx4){0, 0, 0, 0};
         }
     }
     const NibbleMasks mask;
     Q4Block<PER, RT> now;
-    if (first < end) {
-        now.load(a, tile, first, lane);
-    }
+    now.load(a, tile, first, lane);
+    stage(first, shared[0]);
     for (uint32_t b = first; b < end; b++) {
         Q4Block<PER, RT> next = now;
+        __syncthreads();   // this block's planes are there, the other buffer is free
         if (b + 1 < end) {
             next.load(a, tile, b + 1, lane);
+            stage(b + 1, shared[(b + 1 - first) & 1]);
         }
+        const f16x8* planes = shared[(b - first) & 1] + lane;
         f16x8 x[NT][4][2];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                x[n][j][0] = planes[n][((size_t)b * 4 + j) * 128];
-                x[n][j][1] = planes[n][((size_t)b * 4 + j) * 128 + 64];
+                x[n][j][0] = planes[n * 512 + j * 128];
+                x[n][j][1] = planes[n * 512 + j * 128 + 64];
             }
         }
         q4_multiply<PER, RT, NT>(now, x, acc, mask);
         now = next;
     }
-    q4_store<RT, NT>(a, joined, acc, factor, tile, token0);
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const uint32_t token = (tile0 + n) * 16 + (lane & 15);
+        if (token >= a.tokens) {
+            continue;
+        }
+        const float factor = a.factors[token];
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            const uint32_t row = (tile + t) * 16 + 4 * g;
+            if (tile + t >= a.p.tiles) {
+                continue;
+            }
+            floatx4 v = acc[t][n];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                v[i] *= factor;
+            }
+            if (gridDim.z > 1) {
+                const size_t width = (size_t)a.p.tiles * 16;
+                *reinterpret_cast<floatx4*>(a.part +
+                    ((size_t)blockIdx.z * a.tokens + token) * width + row) = v;
+                continue;
+            }
+            float* y = a.y + token * a.y_stride + row;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (row + e < a.p.rows) {
+                    y[e] = v[e];
+                }
+            }
+        }
+    }
 }
 
 // y = the sum of the column splits' parts, in their order.
@@ -486,13 +562,18 @@ extern "C" int lh_launch_q4_quantize(const float* w, uint32_t rows, uint32_t col
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
-// How a product runs. few: planes in the kernel itself. Otherwise nt token tiles a
-// workgroup and `splits` column splits, with scratch for planes, factors and parts.
+// How a product runs. few: planes in the kernel itself, rt row tiles a workgroup.
+// Otherwise nt token tiles a workgroup and `splits` column splits, with scratch for
+// planes, factors and parts.
 struct Q4Plan {
     bool few;
     uint32_t nt, rt, splits, per;
     size_t planes, factors;   // bytes
 };
+
+// Workgroups to aim for, one a unit (down of 45 tokens: 21 us with 256, 25 with 128,
+// 24 with 384); the row tiles of a k_q4_many workgroup.
+enum { Q4_WORKGROUPS = 256, MANY_TILES = 8 };
 
 static Q4Plan q4_plan(uint32_t rows, uint32_t cols, uint32_t tokens)
 {
@@ -501,20 +582,22 @@ static Q4Plan q4_plan(uint32_t rows, uint32_t cols, uint32_t tokens)
     p.per = (blocks + WAVES - 1) / WAVES;
     p.splits = 1;
     p.few = tokens <= 16 && tokens * p.per <= STAGED;
-    // Row tiles of a workgroup: more save reads of x, as long as the chip is full.
-    p.rt = tiles >= 1024 ? 4 : tiles >= 512 ? 2 : 1;
     if (p.few) {
+        // Row tiles of a workgroup: one round of workgroups, two on a unit where their
+        // LDS fits twice.
+        const uint32_t units = q4_few_lds(tokens, p.per, 1) > 80 * 1024 ? 256 : 512;
+        const uint32_t rt = (tiles + units - 1) / units;
+        p.rt = rt < 6 ? rt : 6;
         return p;
     }
     const uint32_t tt = (tokens + 15) / 16;
     p.nt = tt < 4 ? tt : 4;
-    p.rt = tiles >= 512 && p.nt <= 2 ? 4 : 2;   // registers for RT * NT <= 8 tiles
-    const uint32_t groups = (tiles + p.rt - 1) / p.rt * ((tt + p.nt - 1) / p.nt);
-    uint32_t splits = (256 + groups - 1) / groups;
-    const uint32_t most = (blocks + 2 * WAVES - 1) / (2 * WAVES);   // two blocks a wave
+    const uint32_t groups = (tiles + MANY_TILES - 1) / MANY_TILES * ((tt + p.nt - 1) / p.nt);
+    uint32_t splits = (Q4_WORKGROUPS + groups - 1) / groups;
+    const uint32_t most = (blocks + 3) / 4;   // four blocks at least
     splits = splits < most ? splits : most;
-    p.per = (blocks + splits * WAVES - 1) / (splits * WAVES);
-    p.splits = (blocks + p.per * WAVES - 1) / (p.per * WAVES);
+    p.per = (blocks + splits - 1) / splits;
+    p.splits = (blocks + p.per - 1) / p.per;
     p.planes = (size_t)tt * blocks * 8192;
     p.factors = lh_round16((size_t)tokens * 4);
     return p;
@@ -524,10 +607,14 @@ template <int PER>
 static void q4_few(const Q4Plan& p, const Q4Args& a, hipStream_t s)
 {
     const dim3 grid((a.p.tiles + p.rt - 1) / p.rt), block(64 * WAVES);
+    const size_t lds = q4_few_lds(a.tokens, p.per, p.rt);
     switch (p.rt) {
-    case 1: hipLaunchKernelGGL((k_q4_few<PER, 1>), grid, block, 0, s, a); break;
-    case 2: hipLaunchKernelGGL((k_q4_few<PER, 2>), grid, block, 0, s, a); break;
-    default: hipLaunchKernelGGL((k_q4_few<PER, 4>), grid, block, 0, s, a); break;
+    case 1: hipLaunchKernelGGL((k_q4_few<PER, 1>), grid, block, lds, s, a); break;
+    case 2: hipLaunchKernelGGL((k_q4_few<PER, 2>), grid, block, lds, s, a); break;
+    case 3: hipLaunchKernelGGL((k_q4_few<PER, 3>), grid, block, lds, s, a); break;
+    case 4: hipLaunchKernelGGL((k_q4_few<PER, 4>), grid, block, lds, s, a); break;
+    case 5: hipLaunchKernelGGL((k_q4_few<PER, 5>), grid, block, lds, s, a); break;
+    default: hipLaunchKernelGGL((k_q4_few<PER, 6>), grid, block, lds, s, a); break;
     }
 }
 
@@ -535,15 +622,13 @@ template <int PER>
 static void q4_many(const Q4Plan& p, const Q4Args& a, hipStream_t s)
 {
     const uint32_t tt = (a.tokens + 15) / 16;
-    const dim3 grid((a.p.tiles + p.rt - 1) / p.rt, (tt + p.nt - 1) / p.nt, p.splits);
-    const dim3 block(64 * WAVES);
-    switch (p.nt * 8 + p.rt) {
-    case 8 + 2: hipLaunchKernelGGL((k_q4_many<PER, 2, 1>), grid, block, 0, s, a); break;
-    case 8 + 4: hipLaunchKernelGGL((k_q4_many<PER, 4, 1>), grid, block, 0, s, a); break;
-    case 16 + 2: hipLaunchKernelGGL((k_q4_many<PER, 2, 2>), grid, block, 0, s, a); break;
-    case 16 + 4: hipLaunchKernelGGL((k_q4_many<PER, 4, 2>), grid, block, 0, s, a); break;
-    case 24 + 2: hipLaunchKernelGGL((k_q4_many<PER, 2, 3>), grid, block, 0, s, a); break;
-    default: hipLaunchKernelGGL((k_q4_many<PER, 2, 4>), grid, block, 0, s, a); break;
+    const dim3 grid((a.p.tiles + MANY_TILES - 1) / MANY_TILES, (tt + p.nt - 1) / p.nt, p.splits);
+    const dim3 block(256);
+    switch (p.nt) {
+    case 1: hipLaunchKernelGGL((k_q4_many<PER, 1>), grid, block, 0, s, a); break;
+    case 2: hipLaunchKernelGGL((k_q4_many<PER, 2>), grid, block, 0, s, a); break;
+    case 3: hipLaunchKernelGGL((k_q4_many<PER, 3>), grid, block, 0, s, a); break;
+    default: hipLaunchKernelGGL((k_q4_many<PER, 4>), grid, block, 0, s, a); break;
     }
 }
 
@@ -558,15 +643,15 @@ static void q4_product(const Q4Plan& p, const Q4Args& a, hipStream_t s)
 }
 
 // For any number of rows: splits appear below 256 workgroups and bring them to less
-// than 512, of at most four row tiles and (past 64 tokens more workgroups, not more
-// tokens) 64 tokens, so their parts hold at most 512 * 4 * 16 rows of min(tokens, 64).
+// than 512, of eight row tiles and (past 64 tokens more workgroups, not more tokens)
+// 64 tokens, so their parts hold at most 512 * 8 * 16 rows of min(tokens, 64).
 extern "C" size_t lh_q4_scratch_bytes(uint32_t cols, uint32_t tokens)
 {
     const Q4Plan p = q4_plan(1, cols, tokens);
     if (p.few) {
         return 0;
     }
-    const size_t parts = cols > 128 * 2 * WAVES ? (size_t)512 * 4 * 16 * 4 : 0;
+    const size_t parts = cols > 128 * 4 ? (size_t)512 * MANY_TILES * 16 * 4 : 0;
     return p.planes + p.factors + parts * (tokens < 64 ? tokens : 64);
 }
 
@@ -580,7 +665,7 @@ extern "C" int lh_launch_q4_matvec(const uint8_t* packed, const float* x, size_t
     const Q4Args a = {packed, q4_shape(rows, cols, group), x, y, x_stride, y_stride, tokens, p.per,
         planes, factors, reinterpret_cast<float*>(scratch + p.planes + p.factors)};
     if (!p.few) {
-        hipLaunchKernelGGL(k_q4_planes, dim3(tokens), dim3(256), 0, s, a, planes, factors);
+        hipLaunchKernelGGL(k_q4_planes, dim3(tokens), dim3(1024), 0, s, a, planes, factors);
         if (hipGetLastError() != hipSuccess) {
             return -1;
         }
