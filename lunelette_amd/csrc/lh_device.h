@@ -39,13 +39,19 @@ __device__ __forceinline__ uint32_t bf16_nearest(float v)
     return (u + 0x7fffu + ((u >> 16) & 1)) >> 16;
 }
 
-// Four floats from any 4-byte boundary: one 16-byte load, which this chip takes from
-// there (a wave's contiguous words then touch one cache line more).
+// Four floats from and to any 4-byte boundary: one 16-byte access, which this chip
+// makes there (a wave's contiguous words then touch one cache line more).
 __device__ __forceinline__ float4 load4(const float* p)
 {
     typedef float float4_any __attribute__((ext_vector_type(4), aligned(4)));
     const float4_any v = *reinterpret_cast<const float4_any*>(p);
     return make_float4(v.x, v.y, v.z, v.w);
+}
+
+__device__ __forceinline__ void store4(float* p, float4 v)
+{
+    typedef float float4_any __attribute__((ext_vector_type(4), aligned(4)));
+    *reinterpret_cast<float4_any*>(p) = (float4_any){v.x, v.y, v.z, v.w};
 }
 
 // Pairwise halving tree over the 64 lanes of a wave: after the step with
