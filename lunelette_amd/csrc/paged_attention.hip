@@ -19,6 +19,7 @@
 // so a scale is one multiplication for each position and never rounds a value.
 #include "lh_nibbles.h"
 #include "lh_paged.h"
+#include <stdlib.h>
 
 namespace lh {
 
@@ -41,6 +42,20 @@ __device__ __forceinline__ float column_sum(float v)
     const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
         false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// The reference of a column's softmax need not be its maximum: it follows once that is
+// SLACK (in powers of two) above, so the sums are seldom rescaled (with every new
+// maximum some column of a wave had one in most blocks: %s us for the prompt).
+// Probabilities then reach 2^SLACK, their planes 2^SLACK * P_SCALE = 2^14; what a plane
+// drops is below 2^-31 of the reference.
+constexpr float SLACK = 8, P_SCALE = 64;
+
+// The power of two that takes value scales up to `most` below P_SCALE, at most `now`.
+__device__ __forceinline__ float value_shift(float most, float now)
+{
+    const int e = (int)((__float_as_uint(most) >> 23) & 0xffu) - 127;
+    return fminf(now, exp2i(e < -118 ? 123 : 5 - e));
 }
 
 struct AttentionArgs {
@@ -99,147 +114,103 @@ __device__ __forceinline__ void load_query(const float* q, uint32_t g, float sca
     cs = scale * exp2i(-e2);
 }
 
-// A 32-position block's loads: keys as [position tile][..], values, and (Q4) the
-// words of the lane's positions 4 g .. + 3 and 16 + 4 g .. + 3.
+// Prompts: four waves with 32 query rows each (two column tiles) share every block of 32
+// positions in LDS as operands, decoded once by the workgroup: 16 fragments of 64 lanes
+// for 128 dims, keys first, and (Q4) the block's scales and zeros as floats.
 template <int D, bool Q4>
-struct KVBlock {
-    static constexpr int N = Q4 ? D / 64 : D / 16;   // 16-byte words of keys, and of values
-    u32x4 k[N], v[N], ks[2], vs[2];
-
-    __device__ __forceinline__ void load(const uint8_t* part, uint32_t page_size, uint32_t slot,
-        uint32_t lane)
-    {
-        typedef PageLayout<D, Q4> Layout;
-        const uint32_t at = slot * Layout::vector;
-        const u32x4* key = reinterpret_cast<const u32x4*>(part + at);
-        const u32x4* value = reinterpret_cast<const u32x4*>(part + Layout::values(page_size) + at);
-        if (Q4 && D == 64) {
-            // Two 16-position tiles of 8 bytes a lane.
-            const uint2 a = reinterpret_cast<const uint2*>(key)[lane];
-            const uint2 b = reinterpret_cast<const uint2*>(key)[64 + lane];
-            k[0] = (u32x4){a.x, a.y, b.x, b.y};
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                k[i] = key[64 * i + lane];
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            v[i] = value[64 * i + lane];
-        }
-        if (Q4) {
-            const uint32_t g = lane >> 4;
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                ks[t] = *reinterpret_cast<const u32x4*>(part + Layout::scales(page_size, 0) +
-                    4 * (slot + 16 * t + 4 * g));
-                vs[t] = *reinterpret_cast<const u32x4*>(part + Layout::scales(page_size, 1) +
-                    4 * (slot + 16 * t + 4 * g));
-            }
-        }
-    }
-    // Operand of position tile t's dims 32 j .. + 31.
-    __device__ __forceinline__ f16x8 key(int t, int j, const NibbleMasks& mask) const
-    {
-        if (Q4) {
-            const int w = t * (D / 32) + j;
-            return codes_minus8(k[w >> 2][w & 3], mask);
-        }
-        return __builtin_bit_cast(f16x8, k[t * (D / 32) + j]);
-    }
-    __device__ __forceinline__ f16x8 value(int i, const NibbleMasks& mask) const
-    {
-        return Q4 ? codes_minus8(v[i >> 2][i & 3], mask) : __builtin_bit_cast(f16x8, v[i]);
-    }
+struct SharedBlock {
+    f16x8 fragment[D / 8][64];
+    float scale[Q4 ? 4 : 1][32];   // of keys, their zero + 8 scale, of values, theirs
 };
 
-// Running state of a wave's NQ tiles of 16 columns.
-template <int D, bool Q4, int NQ>
-struct Columns {
-    f16x8 hi[NQ][D / 32], lo[NQ][D / 32];   // q in planes
-    float cs[NQ], qs[NQ];     // score factor, sum of the scaled q
-    int32_t limit[NQ];        // last position that the column sees
-    floatx4 acc[NQ][D / 16];  // out^T dims 16 i + 4 g .. + 3, times 2^14 (Q4: shift)
-    float m[NQ], sum[NQ], offset[NQ];   // this lane's parts of the last two
-    bool lost[NQ];
-    int32_t low, high;        // least and largest limit of the wave
-    float shift;              // Q4: 2^(13 - exponent of the largest value scale)
-    NibbleMasks mask;
+template <int D, bool Q4>
+struct PromptRows {
+    f16x8 hi[2][D / 32], lo[2][D / 32];
+    float cs[2], qs[2], m[2], sum[2], offset[2];
+    int32_t limit[2], low, high;
+    floatx4 acc[2][D / 16];
+    float shift;
+    bool lost[2];
+    uint32_t g, lane;
 
-    __device__ __forceinline__ void block(const KVBlock<D, Q4>& b, int32_t base, uint32_t g)
+    __device__ __forceinline__ int32_t position(int32_t base, int e) const
     {
-        const bool edge = base + 31 > low;
-        float ks[8], kz[8], vs[8], vz[8];
-        if (Q4) {
-            float most = 0;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const uint32_t kw = b.ks[e >> 2][e & 3], vw = b.vs[e >> 2][e & 3];
-                ks[e] = bf16_to_f32(kw & 0xffffu);
-                kz[e] = __builtin_fmaf(8.0f, ks[e], __uint_as_float(kw & 0xffff0000u));
-                vs[e] = bf16_to_f32(vw & 0xffffu);
-                vz[e] = __builtin_fmaf(8.0f, vs[e], __uint_as_float(vw & 0xffff0000u));
-                // Places past every column's limit may hold anything.
-                const int32_t p = base + 4 * (int32_t)g + (e & 3) + 16 * (e >> 2);
-                most = fmaxf(most, !edge || p <= high ? vs[e] : 0.0f);
-            }
-            // shift * vs stays below 2^14; a larger scale than so far lowers it.
-            if (__ballot(most * shift >= 16384.0f)) {
-                const float all = column_max(most);
-                const int e = (int)((__float_as_uint(all) >> 23) & 0xffu) - 127;
-                const float next = exp2i(e < -110 ? 123 : 13 - e);
-                const float ratio = next / shift;
-#pragma unroll
-                for (int n = 0; n < NQ; n++) {
-#pragma unroll
-                    for (int i = 0; i < D / 16; i++) {
-                        acc[n][i] *= ratio;
-                    }
-                }
-                shift = next;
-            }
-        }
-        floatx4 s[NQ][2];
+        return base + 4 * (int32_t)g + (e & 3) + 16 * (e >> 2);
+    }
+
+    // The scales `which` and their zeros of the lane's positions.
+    __device__ __forceinline__ void scales(const SharedBlock<D, Q4>& b, int which,
+        float (&scale)[8], float (&z)[8])
+    {
 #pragma unroll
         for (int t = 0; t < 2; t++) {
+            const floatx4 x = *reinterpret_cast<const floatx4*>(
+                &b.scale[Q4 ? which : 0][16 * t + 4 * g]);
+            const floatx4 y = *reinterpret_cast<const floatx4*>(
+                &b.scale[Q4 ? which + 1 : 0][16 * t + 4 * g]);
 #pragma unroll
-            for (int n = 0; n < NQ; n++) {
-                s[n][t] = (floatx4){0, 0, 0, 0};
-            }
-#pragma unroll
-            for (int j = 0; j < D / 32; j++) {
-                const f16x8 k = b.key(t, j, mask);
-#pragma unroll
-                for (int n = 0; n < NQ; n++) {
-                    s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, hi[n][j], s[n][t], 0, 0, 0);
-                    s[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, lo[n][j], s[n][t], 0, 0, 0);
-                }
+            for (int i = 0; i < 4; i++) {
+                scale[4 * t + i] = x[i];
+                z[4 * t + i] = y[i];
             }
         }
-        f16x8 ph[NQ], pl[NQ];
+    }
+
+    __device__ __forceinline__ void block(const SharedBlock<D, Q4>& b, int32_t base)
+    {
+        const bool edge = base + 31 > low;
+        // Fragments are read a step ahead of their products, and products that need one
+        // another stand four apart.
+        floatx4 s[2][2];
+        f16x8 k[2][2];
 #pragma unroll
-        for (int n = 0; n < NQ; n++) {
-            float p[8];
-            uint32_t seen = 0xff;
+        for (int t = 0; t < 2; t++) {
+            k[0][t] = b.fragment[t * (D / 32)][lane];
+            s[0][t] = s[1][t] = (floatx4){0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int j = 0; j < D / 32; j++) {
+#pragma unroll
+            for (int t = 0; t < 2 && j + 1 < D / 32; t++) {
+                k[(j + 1) & 1][t] = b.fragment[t * (D / 32) + j + 1][lane];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                s[x & 1][x >> 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[j & 1][x >> 1],
+                    hi[x & 1][j], s[x & 1][x >> 1], 0, 0, 0);
+            }
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                s[x & 1][x >> 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[j & 1][x >> 1],
+                    lo[x & 1][j], s[x & 1][x >> 1], 0, 0, 0);
+            }
+        }
+        float scale[8], z[8], p[2][8];
+        if (Q4) {
+            scales(b, 0, scale, z);
+        }
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+            float most;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                float v = s[n][e >> 2][e & 3];
-                v = Q4 ? __builtin_fmaf(kz[e], qs[n], ks[e] * v) : v;
-                p[e] = v * cs[n];
+                const float v = s[n][e >> 2][e & 3];
+                p[n][e] = (Q4 ? __builtin_fmaf(z[e], qs[n], scale[e] * v) : v) * cs[n];
             }
             if (edge) {
+                asm volatile("");   // a branch, not selections for every block
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    const bool hidden = base + 4 * (int32_t)g + (e & 3) + 16 * (e >> 2) > limit[n];
-                    p[e] = hidden ? -__builtin_inff() : p[e];
-                    seen &= hidden ? ~(1u << e) : ~0u;
+                    p[n][e] = position(base, e) > limit[n] ? -__builtin_inff() : p[n][e];
                 }
             }
-            float most = fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])),
-                fmaxf(fmaxf(p[4], p[5]), fmaxf(p[6], p[7])));
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                most = e ? fmaxf(most, p[n][e]) : p[n][e];
+            }
             most = fmaxf(column_max(most), m[n]);
-            if (__ballot(most > m[n])) {
+            if (__ballot(most > m[n] + SLACK)) {
                 const float keep = m[n] > -__builtin_inff() ? __builtin_amdgcn_exp2f(m[n] - most)
                     : 0.0f;
                 m[n] = most;
@@ -250,77 +221,135 @@ struct Columns {
                     acc[n][i] *= keep;
                 }
             }
-            const float top = m[n] > -__builtin_inff() ? m[n] : 0.0f;
+        }
+        if (Q4) {
+            scales(b, 2, scale, z);
+            float most = 0;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                p[e] = __builtin_amdgcn_exp2f(p[e] - top);
-                sum[n] += p[e];
-                if (Q4) {
-                    const bool on = !edge || (seen >> e & 1);
-                    offset[n] = __builtin_fmaf(p[e], on ? vz[e] : 0.0f, offset[n]);
-                    p[e] *= on ? vs[e] * shift : 0.0f;
-                } else {
-                    p[e] *= 16384.0f;
-                }
+                most = fmaxf(most, scale[e]);
             }
-            planes8(p, ph[n], pl[n]);
-        }
+            // shift * scale stays below P_SCALE; a larger scale than so far lowers it.
+            if (__ballot(most * shift >= P_SCALE)) {
+                const float next = value_shift(column_max(most), shift), ratio = next / shift;
 #pragma unroll
-        for (int i = 0; i < D / 16; i++) {
-            f16x8 v = b.value(i, mask);
-            if (!Q4 && edge) {
-                // An Inf or NaN at a position that some column does not see (or that
-                // holds no value yet): out of the product, NaN for those that see it.
-                f16x8 odd;
-                bool any = false;
+                for (int n = 0; n < 2; n++) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const bool bad = !__builtin_isfinite((float)v[e]);
-                    const int32_t p = base + 4 * (int32_t)g + (e & 3) + 16 * (e >> 2);
-                    odd[e] = bad && p <= high ? (_Float16)1 : (_Float16)0;
-                    any |= bad && p <= high;
-                    v[e] = bad ? (_Float16)0 : v[e];
-                }
-                if (__ballot(any)) {
-#pragma unroll
-                    for (int n = 0; n < NQ; n++) {
-                        f16x8 on;
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const int32_t p = base + 4 * (int32_t)g + (e & 3) + 16 * (e >> 2);
-                            on[e] = p <= limit[n] ? (_Float16)1 : (_Float16)0;
-                        }
-                        const floatx4 none = {0, 0, 0, 0};
-                        const floatx4 hits = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, on, none,
-                            0, 0, 0);
-#pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            acc[n][i][r] = hits[r] > 0 ? __builtin_nanf("") : acc[n][i][r];
-                        }
+                    for (int i = 0; i < D / 16; i++) {
+                        acc[n][i] *= ratio;
                     }
                 }
+                shift = next;
+            }
+        }
+        f16x8 ph[2], pl[2];
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+            const float top = m[n] > -__builtin_inff() ? m[n] : 0.0f;
+            float vs[8], vz[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                vs[e] = Q4 ? scale[e] * shift : 0.0f;
+                vz[e] = z[e];
+            }
+            if (Q4 && edge) {
+                asm volatile("");
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const bool hidden = position(base, e) > limit[n];
+                    vs[e] = hidden ? 0.0f : vs[e];   // may be a NaN
+                    vz[e] = hidden ? 0.0f : vz[e];
+                }
             }
 #pragma unroll
-            for (int n = 0; n < NQ; n++) {
-                acc[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[n], acc[n][i], 0, 0, 0);
-                acc[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[n], acc[n][i], 0, 0, 0);
+            for (int e = 0; e < 8; e++) {
+                p[n][e] = __builtin_amdgcn_exp2f(p[n][e] - top);
+                sum[n] += p[n][e];
+                if (Q4) {
+                    offset[n] = __builtin_fmaf(p[n][e], vz[e], offset[n]);
+                    p[n][e] *= vs[e];
+                } else {
+                    p[n][e] *= P_SCALE;
+                }
+            }
+            planes8(p[n], ph[n], pl[n]);
+        }
+        f16x8 v[2][2];
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            v[0][x] = b.fragment[D / 16 + x][lane];
+        }
+#pragma unroll
+        for (int i = 0; i < D / 16; i += 2) {
+            const int at = (i / 2) & 1;
+#pragma unroll
+            for (int x = 0; x < 2 && i + 2 < D / 16; x++) {
+                v[at ^ 1][x] = b.fragment[D / 16 + i + 2 + x][lane];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (!Q4 && edge) {
+                v[at][0] = without_odd(v[at][0], i, base);
+                v[at][1] = without_odd(v[at][1], i + 1, base);
+            }
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                acc[x & 1][i + (x >> 1)] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[at][x >> 1],
+                    ph[x & 1], acc[x & 1][i + (x >> 1)], 0, 0, 0);
+            }
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                acc[x & 1][i + (x >> 1)] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[at][x >> 1],
+                    pl[x & 1], acc[x & 1][i + (x >> 1)], 0, 0, 0);
             }
         }
     }
+
+    // v with every Inf or NaN as 0: it may stand at a position that some row does not see,
+    // or that holds no value yet. Rows that see it get NaN.
+    __device__ __forceinline__ f16x8 without_odd(f16x8 v, int i, int32_t base)
+    {
+        f16x8 odd;
+        bool any = false;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const bool bad = !__builtin_isfinite((float)v[e]);
+            odd[e] = bad && position(base, e) <= high ? (_Float16)1 : (_Float16)0;
+            any |= bad && position(base, e) <= high;
+            v[e] = bad ? (_Float16)0 : v[e];
+        }
+        if (__ballot(any)) {
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                f16x8 on;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    on[e] = position(base, e) <= limit[n] ? (_Float16)1 : (_Float16)0;
+                }
+                const floatx4 hits = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, on,
+                    (floatx4){0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    acc[n][i][r] = hits[r] > 0 ? __builtin_nanf("") : acc[n][i][r];
+                }
+            }
+        }
+        return v;
+    }
 };
 
-// Four waves take every fourth block of a split's range for one tile of 16 NQ
-// query rows of a KV head. grid (KV heads, sequences, tiles of the splits in turn): the
-// tiles of a KV head of eight share an XCD and its L2.
-template <int D, bool Q4, int NQ>
-__global__ void __launch_bounds__(256)
-k_paged_attention(AttentionArgs a)
+enum { PROMPT_ROWS = 128 };
+
+// grid (KV heads, sequences, tiles of the splits in turn): the tiles of a KV head of
+// eight share an XCD and its L2. One barrier a block: while a block is multiplied the
+// next one is decoded into the other buffer and the one after is on its way.
+template <int D, bool Q4>
+__global__ void __launch_bounds__(256, 2)
+k_paged_prompt(AttentionArgs a)
 {
-    constexpr int TQ = 16 * NQ, ROW = D + 4;
-    __shared__ float joined[4][TQ][ROW];
-    __shared__ float stats[4][3][TQ];
-    const uint32_t h = blockIdx.x, s = blockIdx.y;
-    const uint32_t lane = threadIdx.x & 63, g = lane >> 4;
+    typedef PageLayout<D, Q4> Layout;
+    constexpr uint32_t LOADERS = D / 32;   // waves that bring four fragments each
+    __shared__ SharedBlock<D, Q4> blocks[2];
+    const uint32_t h = blockIdx.x, s = blockIdx.y, lane = threadIdx.x & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t split = blockIdx.z / a.tiles;
     const Span span = batch_span(a.batch, s);
@@ -328,23 +357,119 @@ k_paged_attention(AttentionArgs a)
     const int64_t capacity = (int64_t)a.batch.width * a.cache.page_size;
     const uint32_t in_page = a.cache.page_size / 32;
     const int32_t* table = a.batch.table + (size_t)s * a.batch.width;
-    const size_t head_bytes = PageLayout<D, Q4>::head_bytes(a.cache.page_size);
-    for (int64_t tile = blockIdx.z % a.tiles; tile * TQ < rows; tile += a.tiles) {
-        Columns<D, Q4, NQ> c;
-        c.low = 0x7fffffff;
-        c.high = -1;
-        c.shift = exp2i(123);
+    const size_t head_bytes = Layout::head_bytes(a.cache.page_size);
+    const NibbleMasks mask;
+    for (int64_t tile = blockIdx.z % a.tiles; tile * PROMPT_ROWS < rows; tile += a.tiles) {
+        auto limit_of = [&](int64_t row) __attribute__((always_inline)) {
+            const int64_t last = span.first + row / a.group;
+            return last < 0 ? -1 : (int32_t)(last < capacity ? last : capacity - 1);
+        };
+        const int64_t last_row = tile * PROMPT_ROWS + PROMPT_ROWS < rows
+            ? tile * PROMPT_ROWS + PROMPT_ROWS - 1 : rows - 1;
+        const int32_t high = limit_of(last_row);
+        const int32_t steps = high < 0 ? 0 : (high >> 6) + 1, all = high < 0 ? 0 : (high >> 5) + 1;
+        const int32_t chunk = split_chunk(a, steps);
+        if (split && (int64_t)split * chunk >= steps) {
+            continue;   // nothing for this split: the join does not ask for it
+        }
+        const int32_t first = 2 * (int32_t)split * chunk;
+        const int32_t end = all - first < 2 * chunk ? all : first + 2 * chunk;
+        PromptRows<D, Q4> c;
+        c.lane = lane;
+        c.g = lane >> 4;
+        // Lane i has the page ids of blocks first + 64 n + i.
+        int32_t ids = 0;
+        u32x4 raw;
+        uint32_t words = 0;
+        bool good = true;
+        auto locate = [&](int32_t b, uint32_t& slot) __attribute__((always_inline)) {
+            const int32_t turn = b - first;
+            if ((turn & 63) == 0) {
+                const int64_t at = (int64_t)((uint64_t)((uint32_t)b + lane) * a.per_page >> 32);
+                ids = at < a.batch.width ? table[at] : -1;
+            }
+            const uint32_t page = (uint32_t)((uint64_t)(uint32_t)b * a.per_page >> 32);
+            int32_t id = __builtin_amdgcn_readlane(ids, turn & 63);
+            good = id >= 0 && (uint32_t)id < a.cache.pages;
+            slot = 32 * ((uint32_t)b - page * in_page);
+            // A block without a place reads page 0 and is lost for the rows that see it.
+            return a.cache.base + ((size_t)(good ? id : 0) * a.cache.kv_heads + h) * head_bytes;
+        };
+        auto missing = [&](int32_t b) __attribute__((always_inline)) {
 #pragma unroll
-        for (int n = 0; n < NQ; n++) {
-            // Columns past the last row repeat it and are not stored.
-            int64_t row = tile * TQ + 16 * n + (lane & 15);
-            row = row < rows ? row : rows - 1;
-            const int64_t t = row / a.group, last = span.first + t;
-            c.lost[n] = last >= capacity;
-            c.limit[n] = last < 0 ? -1 : (int32_t)(last < capacity ? last : capacity - 1);
-            const float* q = a.q + (size_t)(span.begin + t) * a.q_stride +
-                ((size_t)h * a.group + row % a.group) * D;
-            load_query<D>(q, g, a.scale, c.hi[n], c.lo[n], c.cs[n], c.qs[n]);
+            for (int n = 0; n < 2; n++) {
+                c.lost[n] |= !good && 32 * b <= c.limit[n];
+            }
+        };
+        // Q4: asks for block b's words.
+        auto ask = [&](int32_t b) __attribute__((always_inline)) {
+            uint32_t slot;
+            const uint8_t* part = locate(b, slot);
+            missing(b);
+            const uint8_t* key = part + slot * Layout::vector;
+            const uint8_t* value = key + Layout::values(a.cache.page_size);
+            if (wave < LOADERS / 2) {
+                if (D == 64) {
+                    const uint2 x = reinterpret_cast<const uint2*>(key)[lane];
+                    const uint2 y = reinterpret_cast<const uint2*>(key)[64 + lane];
+                    raw = (u32x4){x.x, x.y, y.x, y.y};
+                } else {
+                    raw = reinterpret_cast<const u32x4*>(key)[64 * wave + lane];
+                }
+            } else if (wave < LOADERS) {
+                raw = reinterpret_cast<const u32x4*>(value)[64 * (wave - LOADERS / 2) + lane];
+            }
+            if (wave == 0) {
+                words = *reinterpret_cast<const uint32_t*>(part +
+                    Layout::scales(a.cache.page_size, lane >> 5) + 4 * (slot + (lane & 31)));
+            }
+        };
+        // Q4: block b, asked for before, into `to`.
+        auto decode = [&](int32_t b, SharedBlock<D, Q4>& to) __attribute__((always_inline)) {
+            if (wave < LOADERS) {
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    to.fragment[4 * wave + w][lane] = codes_minus8(raw[w], mask);
+                }
+            }
+            if (wave == 0) {
+                float scale = bf16_to_f32(words & 0xffffu);
+                float z = __builtin_fmaf(8.0f, scale, __uint_as_float(words & 0xffff0000u));
+                if (32 * b + (int32_t)(lane & 31) > high) {
+                    scale = z = 0;   // may hold anything
+                }
+                to.scale[Q4 ? 2 * (lane >> 5) : 0][lane & 31] = scale;
+                to.scale[Q4 ? 2 * (lane >> 5) + 1 : 0][lane & 31] = z;
+            }
+        };
+        // F16: block b straight into `to`.
+        auto fetch = [&](int32_t b, SharedBlock<D, Q4>& to) __attribute__((always_inline)) {
+            uint32_t slot;
+            const uint8_t* part = locate(b, slot);
+            missing(b);
+            const uint8_t* key = part + slot * Layout::vector;
+            const uint8_t* value = key + Layout::values(a.cache.page_size);
+            if (wave < LOADERS) {
+                const uint8_t* from = wave < LOADERS / 2 ? key + 4096 * wave
+                    : value + 4096 * (wave - LOADERS / 2);
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    __builtin_amdgcn_global_load_lds(
+                        (const __attribute__((address_space(1))) void*)(from + 1024 * w + 16 * lane),
+                        (__attribute__((address_space(3))) void*)&to.fragment[4 * wave + w][0], 16,
+                        0, 0);
+                }
+            }
+        };
+        // Rows past the last one repeat it and are not stored.
+        auto row_of = [&](int n) __attribute__((always_inline)) {
+            const int64_t row = tile * PROMPT_ROWS + 32 * wave + 16 * n + (lane & 15);
+            return row < rows ? row : rows - 1;
+        };
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+            c.lost[n] = span.first + row_of(n) / a.group >= capacity;
+            c.limit[n] = limit_of(row_of(n));
             c.m[n] = -__builtin_inff();
             c.sum[n] = c.offset[n] = 0;
 #pragma unroll
@@ -352,89 +477,76 @@ k_paged_attention(AttentionArgs a)
                 c.acc[n][i] = (floatx4){0, 0, 0, 0};
             }
         }
-        // Limits do not fall from a column to the next.
+        c.shift = exp2i(123);
+        // Limits do not fall from a row to the next.
         c.low = __builtin_amdgcn_readlane(c.limit[0], 0);
-        c.high = __builtin_amdgcn_readlane(c.limit[NQ - 1], 15);
-        const int32_t steps = c.high < 0 ? 0 : (c.high >> 6) + 1;
-        const int32_t blocks = c.high < 0 ? 0 : (c.high >> 5) + 1;
-        const int32_t chunk = split_chunk(a, steps);
-        if (split && (int64_t)split * chunk >= steps) {
-            continue;   // nothing for this split: the join does not ask for it
+        c.high = __builtin_amdgcn_readlane(c.limit[1], 15);
+        __syncthreads();   // the previous tile's readers
+        if (first < end) {
+            if constexpr (Q4) {
+                ask(first);
+            } else {
+                fetch(first, blocks[0]);
+            }
         }
-        const int32_t first = 2 * (int32_t)split * chunk;
-        const int32_t end = blocks - first < 2 * chunk ? blocks : first + 2 * chunk;
-        for (int32_t b = first + (int32_t)wave; b < end; b += 4) {
-            const uint32_t page = (uint32_t)((uint64_t)(uint32_t)b * a.per_page >> 32);
-            const int32_t id = __builtin_amdgcn_readfirstlane(table[page]);
-            if (id < 0 || (uint32_t)id >= a.cache.pages) {
 #pragma unroll
-                for (int n = 0; n < NQ; n++) {
-                    c.lost[n] |= 32 * b <= c.limit[n];
+        for (int n = 0; n < 2; n++) {
+            const int64_t row = row_of(n);
+            load_query<D>(a.q + (size_t)(span.begin + row / a.group) * a.q_stride +
+                ((size_t)h * a.group + row % a.group) * D, c.g, a.scale, c.hi[n], c.lo[n], c.cs[n],
+                c.qs[n]);
+        }
+        if (Q4 && first < end) {
+            decode(first, blocks[0]);
+            if (first + 1 < end) {
+                ask(first + 1);
+            }
+        }
+        for (int32_t b = first; b < end; b++) {
+            SharedBlock<D, Q4>&now = blocks[(b - first) & 1], &other = blocks[(b - first + 1) & 1];
+            __syncthreads();   // this block is there, the other buffer is free
+            if (b + 1 < end) {
+                if constexpr (Q4) {
+                    decode(b + 1, other);
+                    if (b + 2 < end) {
+                        ask(b + 2);
+                    }
+                } else {
+                    fetch(b + 1, other);
                 }
+            }
+            if (32 * b <= c.high) {
+                c.block(now, 32 * b);
+            }
+        }
+        const bool whole = steps <= chunk;   // no other split has a part
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+            const float sum = c.lost[n] ? __builtin_nanf("") : column_sum(c.sum[n]);
+            const float offset = column_sum(c.offset[n]);
+            if (tile * PROMPT_ROWS + 32 * wave + 16 * n + (lane & 15) >= rows) {
                 continue;
             }
-            const uint8_t* part = a.cache.base + ((size_t)id * a.cache.kv_heads + h) * head_bytes;
-            KVBlock<D, Q4> kv;
-            kv.load(part, a.cache.page_size, 32 * ((uint32_t)b - page * in_page), lane);
-            c.block(kv, 32 * b, g);
-        }
-        // The four waves' parts: each scales its own to the common maximum.
-        __syncthreads();   // the previous tile's readers
-#pragma unroll
-        for (int n = 0; n < NQ; n++) {
-            const float sum = column_sum(c.sum[n]), offset = column_sum(c.offset[n]);
-            c.sum[n] = c.lost[n] ? __builtin_nanf("") : sum;
-            c.offset[n] = offset;
-            if (g == 0) {
-                stats[wave][0][16 * n + lane] = c.m[n];
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int n = 0; n < NQ; n++) {
-            const uint32_t col = 16 * n + (lane & 15);
-            const float m = fmaxf(fmaxf(stats[0][0][col], stats[1][0][col]),
-                fmaxf(stats[2][0][col], stats[3][0][col]));
-            const float keep = c.m[n] > -__builtin_inff() ? __builtin_amdgcn_exp2f(c.m[n] - m)
-                : 0.0f;
-            // 1 / shift is a power of two.
-            const float back = keep * (Q4 ? 1.0f / c.shift : 1.0f / 16384);
-#pragma unroll
-            for (int i = 0; i < D / 16; i++) {
-                floatx4 v;
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    v[r] = __builtin_fmaf(c.acc[n][i][r], back, Q4 ? c.offset[n] * keep : 0.0f);
-                }
-                *reinterpret_cast<floatx4*>(&joined[wave][col][16 * i + 4 * g]) = v;
-            }
-            if (g == 0) {
-                stats[wave][1][col] = c.lost[n] ? __builtin_nanf("") : c.sum[n] * keep;
-                stats[wave][2][col] = m;
-            }
-        }
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < TQ * D; i += 256) {
-            const uint32_t col = i / D, d = i % D;
-            const int64_t row = tile * TQ + col;
-            if (row >= rows) {
-                break;
-            }
-            const float v = (joined[0][col][d] + joined[1][col][d]) +
-                (joined[2][col][d] + joined[3][col][d]);
-            const float sum = (stats[0][1][col] + stats[1][1][col]) +
-                (stats[2][1][col] + stats[3][1][col]);
+            // (Powers of two; no position at all: 0.)
+            const float back = Q4 ? 1.0f / c.shift : 1.0f / P_SCALE;
+            const float over = whole ? sum == 0 ? 0.0f : 1.0f / sum : 1.0f;
+            const int64_t row = row_of(n);
             const size_t token = (size_t)(span.begin + row / a.group);
             const size_t head = (size_t)h * a.group + row % a.group;
-            if (steps <= chunk) {
-                // No position at all: 0.
-                a.out[token * a.out_stride + head * D + d] = sum == 0 ? 0.0f : v / sum;
-            } else {
-                const size_t at = (token * a.cache.kv_heads * a.group + head) * a.splits + split;
-                a.part[at * D + d] = v;
-                if (d == 0) {
-                    a.tops[at] = make_float2(stats[0][2][col], sum);
+            const size_t at = (token * a.cache.kv_heads * a.group + head) * a.splits + split;
+            float* to = whole ? a.out + token * a.out_stride + head * D : a.part + at * D;
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) {
+                float4 v;
+                float* f = &v.x;
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    f[r] = __builtin_fmaf(c.acc[n][i][r], back, Q4 ? offset : 0.0f) * over;
                 }
+                store4(to + 16 * i + 4 * c.g, v);
+            }
+            if (!whole && c.g == 0) {
+                a.tops[at] = make_float2(c.m[n], sum);
             }
         }
     }
@@ -547,15 +659,26 @@ struct Decode {
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             s[t] = (floatx4){0, 0, 0, 0};
+        }
+        // Products that need one another stand four apart.
 #pragma unroll
-            for (int j = 0; j < D / 32; j++) {
+        for (int j = 0; j < D / 32; j++) {
+            const f16x8 qh = SHARED ? planes[64 * j + at] : hi[SHARED ? 0 : j];
+            const f16x8 ql = SHARED ? planes[64 * (D / 32 + j) + at] : lo[SHARED ? 0 : j];
+            f16x8 x[4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
                 const int w = (t & 1) * (D / 32) + j;
-                const f16x8 x = Q4 ? codes_minus8(step.k[t >> 1][w >> 2][w & 3], mask)
+                x[t] = Q4 ? codes_minus8(step.k[t >> 1][w >> 2][w & 3], mask)
                     : __builtin_bit_cast(f16x8, step.k[t >> 1][Q4 ? 0 : w]);
-                const f16x8 qh = SHARED ? planes[64 * j + at] : hi[SHARED ? 0 : j];
-                const f16x8 ql = SHARED ? planes[64 * (D / 32 + j) + at] : lo[SHARED ? 0 : j];
-                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, qh, s[t], 0, 0, 0);
-                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, ql, s[t], 0, 0, 0);
+            }
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[t], qh, s[t], 0, 0, 0);
+            }
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[t], ql, s[t], 0, 0, 0);
             }
         }
 #pragma unroll
@@ -601,12 +724,10 @@ struct Decode {
                 }
                 most = fmaxf(most, scale[e]);
             }
-            // shift * scale stays below 2^14; a larger scale than so far lowers it.
-            if (__ballot(most * shift >= 16384.0f)) {
+            // shift * scale stays below P_SCALE; a larger scale than so far lowers it.
+            if (__ballot(most * shift >= P_SCALE)) {
                 most = column_max(most);
-                const int e = (int)((__float_as_uint(most) >> 23) & 0xffu) - 127;
-                const float next = fminf(shift, exp2i(e < -110 ? 123 : 13 - e));
-                const float ratio = next / shift;
+                const float next = value_shift(most, shift), ratio = next / shift;
 #pragma unroll
                 for (int i = 0; i < D / 16; i++) {
                     acc[i] *= ratio;
@@ -626,7 +747,7 @@ struct Decode {
             most = fmaxf(most, p[e]);
         }
         most = fmaxf(column_max(most), m);
-        if (__ballot(most > m)) {
+        if (__ballot(most > m + SLACK)) {
             const float keep = m > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - most) : 0.0f;
             m = most;
             sum *= keep;
@@ -645,7 +766,7 @@ struct Decode {
                 offset = __builtin_fmaf(p[e], z[e], offset);
                 p[e] *= scale[e] * shift;
             } else {
-                p[e] *= 16384.0f;
+                p[e] *= P_SCALE;
             }
         }
 #pragma unroll
@@ -877,7 +998,7 @@ k_paged_decode(AttentionArgs a)
             }
         }
         const float keep = c.m > -__builtin_inff() ? __builtin_amdgcn_exp2f(c.m - m) : 0.0f;
-        const float back = keep * (Q4 ? 1.0f / c.shift : 1.0f / 16384);   // powers of two
+        const float back = keep * (Q4 ? 1.0f / c.shift : 1.0f / P_SCALE);   // powers of two
 #pragma unroll
         for (int i = 0; i < D / 16; i++) {
             floatx4 y;
@@ -926,6 +1047,72 @@ k_paged_decode(AttentionArgs a)
     }
 }
 
+// The splits that the tile of row (t, head) had: nothing to join at one.
+__device__ __forceinline__ uint32_t join_splits(const AttentionArgs& a, const Span& span,
+    int64_t t, uint32_t head)
+{
+    const int64_t rows = span.count * a.group;
+    const int64_t capacity = (int64_t)a.batch.width * a.cache.page_size;
+    int64_t end = (t * a.group + head % a.group) / a.tile * a.tile + a.tile;
+    end = end < rows ? end : rows;
+    int64_t last = span.first + (end - 1) / a.group;
+    last = last < capacity ? last : capacity - 1;
+    const int32_t steps = last < 0 ? 0 : (int32_t)(last >> 6) + 1;
+    const int32_t chunk = split_chunk(a, steps);
+    return steps <= chunk ? 1 : (uint32_t)((steps + chunk - 1) / chunk);
+}
+
+// Joins up to FEW_SPLITS splits: D / 4 threads a row, all parts asked for at once.
+enum { FEW_SPLITS = 8 };
+
+template <int D>
+__global__ void __launch_bounds__(256)
+k_paged_join_few(AttentionArgs a)
+{
+    constexpr uint32_t QUADS = D / 4, EACH = 256 / QUADS;
+    const uint32_t s = blockIdx.y, heads = a.cache.kv_heads * a.group;
+    const uint32_t quad = threadIdx.x % QUADS;
+    const Span span = batch_span(a.batch, s);
+    for (int64_t i = (int64_t)blockIdx.x * EACH + threadIdx.x / QUADS; i < span.count * heads;
+         i += (int64_t)gridDim.x * EACH) {
+        const int64_t t = i / heads;
+        const uint32_t head = (uint32_t)(i % heads);
+        const uint32_t splits = join_splits(a, span, t, head);
+        if (splits == 1) {
+            continue;   // written already
+        }
+        const size_t token = (size_t)(span.begin + t), row = (token * heads + head) * a.splits;
+        float2 tops[FEW_SPLITS];
+        float4 part[FEW_SPLITS];
+        float m = -__builtin_inff(), sum = 0;
+        float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (uint32_t x = 0; x < FEW_SPLITS; x++) {
+            const uint32_t at = x < splits ? x : splits - 1;
+            tops[x] = a.tops[row + at];
+            part[x] = reinterpret_cast<const float4*>(a.part)[(row + at) * QUADS + quad];
+            m = fmaxf(m, tops[x].x);
+        }
+#pragma unroll
+        for (uint32_t x = 0; x < FEW_SPLITS; x++) {
+            // A split that saw nothing holds sums of 0, or NaN for a lost position.
+            float keep = tops[x].x > -__builtin_inff() ? __builtin_amdgcn_exp2f(tops[x].x - m)
+                : 1.0f;
+            if (x >= splits) {
+                continue;
+            }
+            sum = __builtin_fmaf(tops[x].y, keep, sum);
+            v.x = __builtin_fmaf(part[x].x, keep, v.x);
+            v.y = __builtin_fmaf(part[x].y, keep, v.y);
+            v.z = __builtin_fmaf(part[x].z, keep, v.z);
+            v.w = __builtin_fmaf(part[x].w, keep, v.w);
+        }
+        const float over = sum == 0 ? 0.0f : 1.0f / sum;
+        store4(a.out + token * a.out_stride + (size_t)head * D + 4 * quad,
+            make_float4(v.x * over, v.y * over, v.z * over, v.w * over));
+    }
+}
+
 // Joins the splits of a (token, head): lane i of every wave weighs splits i, i + 64 ..
 // (at most SPLITS), then 256 / (D / 4) groups of threads take every so many of them,
 // four dims a thread.
@@ -942,20 +1129,11 @@ k_paged_join(AttentionArgs a)
     const uint32_t heads = a.cache.kv_heads * a.group;
     const uint32_t quad = threadIdx.x % QUADS, group = threadIdx.x / QUADS;
     const Span span = batch_span(a.batch, s);
-    const int64_t rows = span.count * a.group;
-    const int64_t capacity = (int64_t)a.batch.width * a.cache.page_size;
     for (int64_t t = blockIdx.y; t < span.count; t += gridDim.y) {
-        // The splits that the row's tile had.
-        int64_t end = (t * a.group + head % a.group) / a.tile * a.tile + a.tile;
-        end = end < rows ? end : rows;
-        int64_t last = span.first + (end - 1) / a.group;
-        last = last < capacity ? last : capacity - 1;
-        const int32_t steps = last < 0 ? 0 : (int32_t)(last >> 6) + 1;
-        const int32_t chunk = split_chunk(a, steps);
-        if (steps <= chunk) {
+        const uint32_t splits = join_splits(a, span, t, head);
+        if (splits == 1) {
             continue;   // written already
         }
-        const uint32_t splits = (uint32_t)((steps + chunk - 1) / chunk);
         const size_t token = (size_t)(span.begin + t), row = (token * heads + head) * a.splits;
         float2 tops[SPLITS / 64];
         float m = -__builtin_inff(), sum = 0;
@@ -1027,18 +1205,23 @@ static AttentionPlan attention_plan(const lh_paged_cache* c, const lh_paged_batc
     const uint64_t query = b->max_query < b->tokens ? b->max_query : b->tokens;
     const uint64_t rows = query * group;
     AttentionPlan p;
-    p.tile = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+    p.tile = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 32 ? 16 : PROMPT_ROWS;
     const uint64_t tiles = (rows + p.tile - 1) / p.tile;
     p.tiles = (uint32_t)(tiles < 1024 ? tiles : 1024);
     uint64_t longest = (uint64_t)b->table_width * c->page_size;
     longest = b->max_length < longest ? b->max_length : longest;
     const uint64_t steps = (longest + 63) / 64;
+    const uint64_t PRES = getenv("PRES") ? atoi(getenv("PRES")) : 512;
     const uint64_t all = tiles * c->kv_heads * b->sequences * steps;
     uint64_t chunk = (all + RESIDENT - 1) / RESIDENT;
     chunk = chunk < MIN_CHUNK ? MIN_CHUNK : chunk;
     if (chunk > FULL_CHUNK) {
         chunk = (all + WORKGROUPS - 1) / WORKGROUPS;
         chunk = chunk < FULL_CHUNK ? FULL_CHUNK : chunk;
+    }
+    if (p.tile == PROMPT_ROWS) {
+        chunk = (all + PRES - 1) / PRES;
+        chunk = chunk < 4 ? 4 : chunk;
     }
     const uint64_t most = 65535 / p.tiles < SPLITS ? 65535 / p.tiles : SPLITS;
     uint64_t splits = (steps + chunk - 1) / chunk;
@@ -1067,10 +1250,16 @@ static void attention(const lh_paged_cache* c, const lh_paged_batch* b, const At
     case 4: hipLaunchKernelGGL((k_paged_decode<D, Q4, 4>), grid, block, 0, s, a); break;
     case 8: hipLaunchKernelGGL((k_paged_decode<D, Q4, 8>), grid, block, 0, s, a); break;
     case 16: hipLaunchKernelGGL((k_paged_decode<D, Q4, 16>), grid, block, 0, s, a); break;
-    default: hipLaunchKernelGGL((k_paged_attention<D, Q4, 2>), grid, block, 0, s, a); break;
+    default: hipLaunchKernelGGL((k_paged_prompt<D, Q4>), grid, block, 0, s, a); break;
     }
     if (p.splits > 1) {
         const uint32_t query = b->max_query < b->tokens ? b->max_query : b->tokens;
+        const uint64_t each = (uint64_t)query * c->kv_heads * a.group * D / 1024;
+        if (p.splits <= FEW_SPLITS) {
+            hipLaunchKernelGGL((k_paged_join_few<D>), dim3(each < 1 ? 1 : each > 4096 ? 4096 : each,
+                b->sequences), block, 0, s, a);
+            return;
+        }
         hipLaunchKernelGGL((k_paged_join<D>), dim3(c->kv_heads * a.group,
             query < 65535 ? query : 65535, b->sequences), block, 0, s, a);
     }
