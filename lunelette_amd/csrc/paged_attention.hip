@@ -196,7 +196,7 @@ struct PromptRows {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const float v = s[n][e >> 2][e & 3];
-                p[n][e] = (Q4 ? __builtin_fmaf(z[e], qs[n], scale[e] * v) : v) * cs[n];
+                p[n][e] = Q4 ? __builtin_fmaf(z[e], qs[n], scale[e] * v) : v;
             }
             if (edge) {
                 asm volatile("");   // a branch, not selections for every block
@@ -209,7 +209,7 @@ struct PromptRows {
             for (int e = 0; e < 8; e++) {
                 most = e ? fmaxf(most, p[n][e]) : p[n][e];
             }
-            most = fmaxf(column_max(most), m[n]);
+            most = fmaxf(column_max(most) * cs[n], m[n]);
             if (__ballot(most > m[n] + SLACK)) {
                 const float keep = m[n] > -__builtin_inff() ? __builtin_amdgcn_exp2f(m[n] - most)
                     : 0.0f;
@@ -263,7 +263,7 @@ struct PromptRows {
             }
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                p[n][e] = __builtin_amdgcn_exp2f(p[n][e] - top);
+                p[n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[n][e], cs[n], -top));
                 sum[n] += p[n][e];
                 if (Q4) {
                     offset[n] = __builtin_fmaf(p[n][e], vz[e], offset[n]);
@@ -648,7 +648,7 @@ struct Decode {
         return base + 16 * (PACK * (e >> 2) + (int32_t)u) + 4 * (int32_t)g + (e & 3);
     }
 
-    // Scores of the lane's positions, in units of 2: s * scale * log2 e.
+    // Scores of the lane's positions, in units of 1 / cs.
     __device__ __forceinline__ void scores(const Step& step, float (&p)[C])
     {
         floatx4 s[4];
@@ -701,7 +701,7 @@ struct Decode {
                         __uint_as_float(word & 0xffff0000u));
                     y = __builtin_fmaf(z, qs, scale * y);
                 }
-                p[4 * w + i] = y * cs;
+                p[4 * w + i] = y;
             }
         }
     }
@@ -746,7 +746,7 @@ struct Decode {
         for (int e = 1; e < C; e++) {
             most = fmaxf(most, p[e]);
         }
-        most = fmaxf(column_max(most), m);
+        most = fmaxf(column_max(most) * cs, m);
         if (__ballot(most > m + SLACK)) {
             const float keep = m > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - most) : 0.0f;
             m = most;
@@ -760,7 +760,7 @@ struct Decode {
         const float top = m > -__builtin_inff() ? m : 0.0f;
 #pragma unroll
         for (int e = 0; e < C; e++) {
-            p[e] = __builtin_amdgcn_exp2f(p[e] - top);
+            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[e], cs, -top));
             sum += p[e];
             if (Q4) {
                 offset = __builtin_fmaf(p[e], z[e], offset);
@@ -942,19 +942,19 @@ k_paged_decode(AttentionArgs a)
         }
         int32_t turn = 0;
         if constexpr (Q4) {
-            // A step is little: the next one's loads run during all of this one.
+            // A step is little: the next one's loads run during all of this one (the last
+            // one asks for itself again, which spares every step a selection).
             while (x < end) {
                 const int32_t base = 64 * x;
-                const bool edge = base + 63 > c.low;
+                const bool edge = base + 63 > c.low, more = x + 4 < end;
                 float p[C];
                 uint32_t ph[C / 2], pl[C / 2];
-                DecodeStep<D, Q4, C> next = step;
+                DecodeStep<D, Q4, C> next;
+                turn += more ? 1 : 0;
+                locate(more ? x + 4 : x, turn);
+                keys(next);
+                values(next);
                 x += 4;
-                if (x < end) {
-                    locate(x, ++turn);
-                    keys(next);
-                    values(next);
-                }
                 c.scores(step, p);
                 c.probabilities(step, p, base, edge, ph, pl);
                 c.products(step, ph, pl, base, edge);
