@@ -19,7 +19,6 @@
 // so a scale is one multiplication for each position and never rounds a value.
 #include "lh_nibbles.h"
 #include "lh_paged.h"
-#include <stdlib.h>
 
 namespace lh {
 
@@ -46,7 +45,8 @@ __device__ __forceinline__ float column_sum(float v)
 
 // The reference of a column's softmax need not be its maximum: it follows once that is
 // SLACK (in powers of two) above, so the sums are seldom rescaled (with every new
-// maximum some column of a wave had one in most blocks: %s us for the prompt).
+// maximum some column of a wave had one in most blocks: 62.6 against 57.1 us for 256
+// tokens after 4096 positions).
 // Probabilities then reach 2^SLACK, their planes 2^SLACK * P_SCALE = 2^14; what a plane
 // drops is below 2^-31 of the reference.
 constexpr float SLACK = 8, P_SCALE = 64;
@@ -111,7 +111,8 @@ __device__ __forceinline__ void load_query(const float* q, uint32_t g, float sca
         planes8(v + 8 * j, hi[j], lo[j]);
     }
     qs = column_sum(sum);
-    cs = scale * exp2i(-e2);
+    // Never 0 or Inf, which an infinite or a zero score would turn into NaN.
+    cs = fminf(fmaxf(scale * exp2i(-e2), 1e-37f), 3e38f);
 }
 
 // Prompts: four waves with 32 query rows each (two column tiles) share every block of 32
@@ -1189,11 +1190,15 @@ using namespace lh;
 
 // How the steps are split. RESIDENT workgroups are on the chip at once; up to them a
 // split takes as few as MIN_CHUNK steps (one sequence of 16000 positions: 13.7 us with
-// 8, 15.8 with 4, 16.5 with 16). Past them FULL_CHUNK at least, which pays for a
-// workgroup's start (32 sequences up to 4352 in FP16: 36 us with 16, 41 with 8), and about
+// 8, 15.4 with 4, 14.7 with 12). Past them FULL_CHUNK at least, which pays for a
+// workgroup's start (32 sequences up to 4352 in FP16: 30 us with 12 or 16, 33 with 24), and about
 // WORKGROUPS in all, so that sequences of other lengths than the bound spread evenly
-// (64 up to 17920 in 4 bits: 106 us with 2048, 127 with 512, 122 with 8192).
-enum { RESIDENT = 512, WORKGROUPS = 2048, MIN_CHUNK = 8, FULL_CHUNK = 16 };
+// (64 up to 17920 in 4 bits: 102 us with 1024, 103 with 2048, 127 with 512, 122 with 8192).
+// A workgroup of a prompt has 128 rows, and the splits' parts are as large as its output
+// for each: PROMPT_WORKGROUPS in all (256 tokens after 4096 positions: 57 us with 512,
+// 68 with 256, 118 with 128), PROMPT_CHUNK steps at least.
+enum { RESIDENT = 512, WORKGROUPS = 2048, MIN_CHUNK = 8, FULL_CHUNK = 16,
+    PROMPT_WORKGROUPS = 512, PROMPT_CHUNK = 4 };
 
 struct AttentionPlan {
     uint32_t tile, tiles, splits, chunk;
@@ -1205,13 +1210,15 @@ static AttentionPlan attention_plan(const lh_paged_cache* c, const lh_paged_batc
     const uint64_t query = b->max_query < b->tokens ? b->max_query : b->tokens;
     const uint64_t rows = query * group;
     AttentionPlan p;
+    // The least tile that has all rows of a sequence, to 32 (8 sequences up to 4352 in 4
+    // bits and in FP16, group 4: 4 tokens take 29 and 32 us, the prompts' 46 and 42; 8 take
+    // 34 and 36 against 47 and 43; 16 take 50 and 51 against 49 and 45).
     p.tile = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 32 ? 16 : PROMPT_ROWS;
     const uint64_t tiles = (rows + p.tile - 1) / p.tile;
     p.tiles = (uint32_t)(tiles < 1024 ? tiles : 1024);
     uint64_t longest = (uint64_t)b->table_width * c->page_size;
     longest = b->max_length < longest ? b->max_length : longest;
     const uint64_t steps = (longest + 63) / 64;
-    const uint64_t PRES = getenv("PRES") ? atoi(getenv("PRES")) : 512;
     const uint64_t all = tiles * c->kv_heads * b->sequences * steps;
     uint64_t chunk = (all + RESIDENT - 1) / RESIDENT;
     chunk = chunk < MIN_CHUNK ? MIN_CHUNK : chunk;
@@ -1220,8 +1227,8 @@ static AttentionPlan attention_plan(const lh_paged_cache* c, const lh_paged_batc
         chunk = chunk < FULL_CHUNK ? FULL_CHUNK : chunk;
     }
     if (p.tile == PROMPT_ROWS) {
-        chunk = (all + PRES - 1) / PRES;
-        chunk = chunk < 4 ? 4 : chunk;
+        chunk = (all + PROMPT_WORKGROUPS - 1) / PROMPT_WORKGROUPS;
+        chunk = chunk < PROMPT_CHUNK ? PROMPT_CHUNK : chunk;
     }
     const uint64_t most = 65535 / p.tiles < SPLITS ? 65535 / p.tiles : SPLITS;
     uint64_t splits = (steps + chunk - 1) / chunk;
