@@ -108,10 +108,14 @@ k_q4_quantize(const float* __restrict__ w, Q4Shape p, uint8_t* __restrict__ pack
 
 // The product. A wave takes 128-column blocks of RT row tiles for NT tiles of 16
 // tokens: y^T tile [16 rows][16 tokens] = W X^T by 16x16x32 FP16 matrix instructions,
-// W the codes minus 8 (exact), X two planes h + l of x times a power of two. A
-// group's sums are formed from 0 and join the row's by its scale in FP32, so a scale
-// never rounds a weight. Eight waves split the columns and meet in LDS. Codes and
-// scales of the next block are on their way while one is multiplied.
+// W the codes minus 8 (exact), X two planes h + l of x times a power of two: 22 bits of
+// the largest x that shares the power (of a token's 128 columns; all of its columns past
+// SOME_TOKENS). A group's sums are formed from 0 and join the row's by its scale in FP32,
+// so a scale never rounds a weight. Codes and scales of the blocks to come are on their
+// way while one is multiplied.
+// Bound: the codes' bytes. Measured, cold weights: 131072 x 3072 (214 MB) for one token
+// 50 us, 4.3 TB/s, for eight 54 us; 18432 x 3072 with groups of 32 (32 MB) 14 us for one
+// token and for eight, 16 to 18 for 16, of which a launch and the first bytes' way are 5.
 enum { WAVES = 8 };
 
 struct Q4Args {
@@ -123,7 +127,7 @@ struct Q4Args {
     uint32_t tokens, per;       // per: blocks of a wave
     const f16x8* planes;        // [token tile][block][32-column step][plane][lane]
     const float* factors;       // [token]: the power of two back
-    float* part;                // [split][token][16 tiles] where blockIdx.z splits
+    float* part;                // [split][token][16 tiles] where columns are split
 };
 
 // A block's codes and scales of RT tiles. PER: scales of a row in a block.
@@ -188,166 +192,398 @@ __device__ __forceinline__ void q4_multiply(const Q4Block<PER, RT>& b, const f16
     }
 }
 
-// The eight waves' sums of RT tiles (each times its factor) to y.
-template <int RT>
-__device__ __forceinline__ void q4_store(const Q4Args& a, floatx4* joined,
-    const floatx4 (&acc)[RT][1], float factor, uint32_t tile)
+// The same of one block whose token columns have powers of two of their own: f[n] takes
+// the block's sums back, in FP32 (a product with a power of two is exact). x(n, j, plane)
+// reads an operand when it is needed.
+template <int PER, int RT, int NT, class X>
+__device__ __forceinline__ void q4_multiply_block(const Q4Block<PER, RT>& b, const X& x,
+    const float (&f)[NT], floatx4 (&acc)[RT][NT], const NibbleMasks& mask)
 {
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int STEPS = 4 / PER;   // 32-column steps of a group
+    floatx4 sum[RT][NT], d[RT][NT];
 #pragma unroll
-    for (int t = 0; t < RT; t++) {
-        floatx4 v = acc[t][0];
+    for (int j = 0; j < 4; j++) {
+        f16x8 w[RT];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v[i] *= factor;
+        for (int t = 0; t < RT; t++) {
+            w[t] = codes_minus8(b.w[t][j], mask);
         }
-        joined[(t * WAVES + wave) * 64 + lane] = v;
-    }
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < RT * 64; i += 64 * WAVES) {
-        const uint32_t l = i & 63, t = i >> 6;
-        floatx4 v = joined[t * WAVES * 64 + l];
 #pragma unroll
-        for (int w = 1; w < WAVES; w++) {
-            v += joined[(t * WAVES + w) * 64 + l];
+        for (int n = 0; n < NT; n++) {
+            const f16x8 high = x(n, j, 0), low = x(n, j, 1);
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                if (j % STEPS == 0) {
+                    d[t][n] = (floatx4){0, 0, 0, 0};
+                }
+                d[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[t], high, d[t][n], 0, 0, 0);
+                d[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[t], low, d[t][n], 0, 0, 0);
+            }
         }
-        const uint32_t token = l & 15, row = (tile + t) * 16 + 4 * (l >> 4);
-        if (token >= a.tokens) {
+        if (j % STEPS != STEPS - 1) {
             continue;
         }
-        float* y = a.y + token * a.y_stride + row;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (row + e < a.p.rows) {
-                y[e] = v[e];
+        for (int t = 0; t < RT; t++) {
+            const uint32_t low = b.s[t][2 * (j / STEPS)], high = b.s[t][2 * (j / STEPS) + 1];
+            const float s[4] = {bf16_to_f32(low & 0xffffu), __uint_as_float(low & 0xffff0000u),
+                bf16_to_f32(high & 0xffffu), __uint_as_float(high & 0xffff0000u)};
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if constexpr (PER * RT * NT > 24) {
+                        // No registers for a block's sums.
+                        acc[t][n][i] = __builtin_fmaf(s[i] * f[n], d[t][n][i], acc[t][n][i]);
+                        continue;
+                    }
+                    sum[t][n][i] = j < STEPS ? s[i] * d[t][n][i]
+                        : __builtin_fmaf(s[i], d[t][n][i], sum[t][n][i]);
+                    if (j == 3) {
+                        acc[t][n][i] = __builtin_fmaf(f[n], sum[t][n][i], acc[t][n][i]);
+                    }
+                }
             }
         }
     }
 }
 
-// Few tokens: every wave turns its own columns of x into planes in LDS first (its own
-// power of two for each token), with the first block's codes on their way. At most
-// STAGED (token, block) pairs a wave, 512 bytes each; no scratch and one launch.
-enum { STAGED = 32 };
-
-// LDS: the planes, then the waves' sums.
-static size_t q4_few_lds(uint32_t tokens, uint32_t per, uint32_t rt)
+// Four rows of a token: to y, or to the split's part.
+__device__ __forceinline__ void q4_put(const Q4Args& a, floatx4 v, uint32_t token, uint32_t row,
+    uint32_t split, uint32_t splits)
 {
-    const size_t planes = (size_t)WAVES * tokens * per * 512, sums = (size_t)rt * WAVES * 1024;
-    return planes > sums ? planes : sums;
+    if (splits > 1) {
+        *reinterpret_cast<floatx4*>(a.part +
+            ((size_t)split * a.tokens + token) * a.p.tiles * 16 + row) = v;
+        return;
+    }
+    float* y = a.y + token * a.y_stride + row;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        if (row + e < a.p.rows) {
+            y[e] = v[e];
+        }
+    }
 }
 
-template <int PER, int RT>
+__device__ __forceinline__ void load_chunk(const float* x, float (&v)[8])
+{
+    const float4 p = load4(x), q = load4(x + 4);
+    v[0] = p.x, v[1] = p.y, v[2] = p.z, v[3] = p.w;
+    v[4] = q.x, v[5] = q.y, v[6] = q.z, v[7] = q.w;
+}
+
+// Planes of a token's chunk of eight columns (0 if it has none), where 16 lanes side by
+// side have those of a block; its power of two back.
+__device__ __forceinline__ float chunk_planes(float (&v)[8], bool used, f16x8& hi, f16x8& lo)
+{
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        v[e] = used ? v[e] : 0.0f;
+    }
+    uint32_t m = 0;   // magnitudes order as their bits; an Inf or NaN is the largest
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const uint32_t bits = __float_as_uint(v[e]) & 0x7fffffffu;
+        m = m > bits ? m : bits;
+    }
+    uint32_t o;   // the row's other lanes by rotations of 8, 4, 2 and 1
+    o = (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x128, 0xf, 0xf, false), m = m > o ? m : o;
+    o = (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x124, 0xf, 0xf, false), m = m > o ? m : o;
+    o = (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x122, 0xf, 0xf, false), m = m > o ? m : o;
+    o = (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x121, 0xf, 0xf, false), m = m > o ? m : o;
+    const int e2 = row_exponent(__uint_as_float(m));
+    const float up = exp2i(e2);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        v[e] *= up;
+    }
+    planes8(v, hi, lo);
+    return exp2i(-e2);
+}
+
+// Few tokens: every wave turns its own columns of x into planes in LDS first, with the
+// first DEPTH blocks' codes on their way, then takes row tiles in turn: the codes of
+// the blocks to come, of the next tiles too, stay DEPTH ahead. At most STAGED (token,
+// block) pairs a wave; no scratch and one launch.
+// A pair's 512 bytes of planes are followed by 16 with its power of two back, which
+// shifts the next token's to other banks.
+enum { STAGED = 32, PAIR = 33 };   // PAIR: f16x8 of one
+
+static size_t q4_few_lds(uint32_t tokens, uint32_t per, uint32_t rt)
+{
+    // The waves' sums of two turns, then the pairs.
+    return (size_t)2 * rt * WAVES * 1024 + (size_t)WAVES * tokens * per * PAIR * 16;
+}
+
+template <int PER, int RT, int DEPTH>
 __global__ void __launch_bounds__(64 * WAVES)
 k_q4_few(Q4Args a)
 {
     extern __shared__ floatx4 shared[];
-    __shared__ uint32_t most[WAVES][16];
-    const uint32_t lane = threadIdx.x & 63, g = lane >> 4;
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, tokens = a.tokens;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t tile = blockIdx.x * RT, tokens = a.tokens;
     const uint32_t first = wave * a.per;
-    // [block][step][plane][g][token]
-    f16x8* planes = reinterpret_cast<f16x8*>(shared) + wave * tokens * a.per * 32;
-    const uint32_t end = first + a.per < a.p.blocks ? first + a.per : a.p.blocks;
-    // Chunks of eight columns: lane l takes chunks l, l + 64 .. of (token, chunk).
-    constexpr int EACH = STAGED / 4;
-    const uint32_t width = a.per * 16, used = tokens * width;
-    const float inverse = 1.0f / (float)width;
-    float v[EACH][8];
-    uint32_t token[EACH], chunk[EACH];
-    if (lane < 16) {
-        most[wave][lane] = 0;
-    }
-#pragma unroll
-    for (int i = 0; i < EACH; i++) {
-        if (64u * i >= used) {
-            break;
+    const uint32_t left = first < a.p.blocks ? a.p.blocks - first : 0;
+    const uint32_t blocks = left < a.per ? left : a.per;
+    floatx4* joined = shared;   // [turn][tile][wave][lane]
+    // [block][token][step][plane][g] of the wave
+    f16x8* planes = reinterpret_cast<f16x8*>(shared + 2 * RT * WAVES * 64) +
+        wave * tokens * a.per * PAIR;
+    const uint32_t pairs = tokens * blocks, stride = gridDim.x * RT;
+    const float inverse = 1.0f / (float)tokens;
+    Q4Block<PER, RT> ring[DEPTH];
+    uint32_t load_tile = blockIdx.x * RT, load_block = 0;
+    // Unconditional, as all loads here: after one that may not have been issued the
+    // compiler can only wait for everything. Past the end the last tile comes again, a
+    // wave without columns takes those of the first block and drops them.
+    auto ask = [&](Q4Block<PER, RT>& to) __attribute__((always_inline)) {
+        to.load(a, load_tile, blocks ? first + load_block : 0, lane);
+        if (++load_block >= blocks) {
+            load_block = 0;
+            load_tile += load_tile + stride < a.p.tiles ? stride : 0;
         }
-        const uint32_t id = 64 * i + lane;
-        token[i] = (uint32_t)(((float)id + 0.5f) * inverse);   // exact: ids are below 2^10
-        chunk[i] = id - token[i] * width;
-        const uint32_t col = first * 128 + chunk[i] * 8;
-        if (token[i] < tokens && col < a.p.cols) {
-            const float* x = a.x + token[i] * a.x_stride + col;
-            const float4 p = load4(x), q = load4(x + 4);
-            v[i][0] = p.x, v[i][1] = p.y, v[i][2] = p.z, v[i][3] = p.w;
-            v[i][4] = q.x, v[i][5] = q.y, v[i][6] = q.z, v[i][7] = q.w;
-        } else {
+    };
+    float v[4][8];
+    bool used[4];
+    auto load_x = [&](uint32_t base) __attribute__((always_inline)) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                v[i][e] = 0;
-            }
+        for (int i = 0; i < 4; i++) {
+            const uint32_t pair = base + 4 * i + g;
+            // Exact: pairs are below 2^10.
+            const uint32_t block = (uint32_t)(((float)pair + 0.5f) * inverse);
+            const uint32_t token = pair - block * tokens;
+            const uint32_t col = (first + block) * 128 + (lane & 15) * 8;
+            used[i] = pair < pairs && col < a.p.cols;
+            load_chunk(a.x + (used[i] ? token * a.x_stride + col : 0), v[i]);
         }
-    }
-    Q4Block<PER, RT> now;
-    if (first < end) {
-        now.load(a, tile, first, lane);
-    }
+    };
+    auto make = [&](uint32_t base) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < EACH; i++) {
-        if (64u * i >= used) {
-            break;
-        }
-        uint32_t m = 0;   // magnitudes order as their bits; an Inf or NaN is the largest
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const uint32_t bits = __float_as_uint(v[i][e]) & 0x7fffffffu;
-            m = m > bits ? m : bits;
-        }
-        if (token[i] < tokens) {
-            atomicMax(&most[wave][token[i]], m);
-        }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < EACH; i++) {
-        if (64u * i >= used) {
-            break;
-        }
-        if (token[i] < tokens) {
-            const float up = exp2i(row_exponent(__uint_as_float(most[wave][token[i]])));
-            float s[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                s[e] = v[i][e] * up;
-            }
+        for (int i = 0; i < 4; i++) {
             f16x8 hi, lo;
-            planes8(s, hi, lo);
-            // Chunk: block, step j and g in turn.
-            f16x8* to = planes + ((chunk[i] >> 2) * 8 + (chunk[i] & 3)) * tokens + token[i];
-            to[0] = hi;
-            to[4 * tokens] = lo;
+            const float back = chunk_planes(v[i], used[i], hi, lo);
+            const uint32_t pair = base + 4 * i + g;
+            if (pair < pairs) {
+                // Chunk: step j and g in turn.
+                f16x8* to = planes + pair * PAIR + (lane & 12) * 2 + (lane & 3);
+                to[0] = hi;
+                to[4] = lo;
+                if ((lane & 15) == 0) {
+                    *reinterpret_cast<float*>(planes + pair * PAIR + 32) = back;
+                }
+            }
         }
+    };
+    load_x(0);
+#pragma unroll
+    for (int d = 0; d < DEPTH; d++) {
+        __builtin_amdgcn_sched_barrier(0);   // in their order, which the waits go by
+        ask(ring[d]);
     }
-    __syncthreads();
+    make(0);
+    for (uint32_t base = 16; base < pairs; base += 16) {
+        load_x(base);
+        make(base);
+    }
+    // Only this wave reads them.
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
     const NibbleMasks mask;
     const uint32_t mine = (lane & 15) < tokens ? lane & 15 : tokens - 1;
-    float factor[1] = {exp2i(-row_exponent(__uint_as_float(most[wave][mine])))};
+    const f16x8* planes_mine = planes + mine * PAIR;
+    uint32_t tile = blockIdx.x * RT, block = 0;
     floatx4 acc[RT][1];
 #pragma unroll
     for (int t = 0; t < RT; t++) {
         acc[t][0] = (floatx4){0, 0, 0, 0};
     }
-    for (uint32_t b = first; b < end; b++) {
-        Q4Block<PER, RT> next = now;
-        if (b + 1 < end) {
-            next.load(a, tile, b + 1, lane);
+    // The eight waves' sums of the tiles to y.
+    auto store = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            joined[(t * WAVES + wave) * 64 + lane] = acc[t][0];
+            acc[t][0] = (floatx4){0, 0, 0, 0};
         }
-        f16x8 x[1][4][2];
+        // Waits for LDS alone, not for the codes on their way. The next turn writes the
+        // other half; by the one after it all have read this one.
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+        if (wave < RT) {
+            floatx4 v = joined[wave * WAVES * 64 + lane];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+            for (int w = 1; w < WAVES; w++) {
+                v += joined[(wave * WAVES + w) * 64 + lane];
+            }
+            const uint32_t token = lane & 15, row = (tile + wave) * 16 + 4 * g;
+            float* y = a.y + token * a.y_stride + row;
 #pragma unroll
-            for (int plane = 0; plane < 2; plane++) {
-                x[0][j][plane] = planes[(((b - first) * 4 + j) * 8 + plane * 4 + g) * tokens +
-                    mine];
+            for (int e = 0; e < 4; e++) {
+                if (token < tokens && row + e < a.p.rows) {
+                    y[e] = v[e];
+                }
             }
         }
-        q4_multiply<PER, RT, 1>(now, x, acc, mask);
-        now = next;
+        joined = joined == shared ? shared + RT * WAVES * 64 : shared;
+        tile += stride;
+    };
+    if (blocks == 0) {
+        while (tile < a.p.tiles) {
+            store();
+        }
+        return;
     }
-    __syncthreads();   // the planes are done with
-    q4_store<RT>(a, shared, acc, factor[0], tile);
+    while (true) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; d++) {
+            const f16x8* pair = planes_mine + block * tokens * PAIR;
+            auto x = [&](int, int j, int plane) __attribute__((always_inline)) {
+                return pair[j * 8 + plane * 4 + g];
+            };
+            const float f[1] = {*reinterpret_cast<const float*>(pair + 32)};
+            q4_multiply_block<PER, RT, 1>(ring[d], x, f, acc, mask);
+            // The scales are done with before they are loaded over: moved to registers of
+            // their own, the loop's end would wait for the loads to move them back.
+            __builtin_amdgcn_sched_barrier(0);
+            ask(ring[d]);
+            if (++block == blocks) {
+                store();
+                block = 0;
+                if (tile >= a.p.tiles) {
+                    return;
+                }
+            }
+        }
+    }
+}
+
+// Up to 64 tokens: eight waves, two row tiles each, in two halves that take every
+// second block. The blocks' planes are shared in LDS, made for the next two blocks while
+// two are multiplied, with codes two turns ahead. grid (8-tile row groups, column
+// splits). Token t of step j's g is at place (t + g + 4 j) % 16 of its sixteen, so that
+// a token's sixteen chunks go to different banks.
+template <int PER, int NT>
+__global__ void __launch_bounds__(512)
+k_q4_some(Q4Args a)
+{
+    constexpr int RT = 2, BLOCK = NT * 512;   // f16x8 of a block's planes
+    extern __shared__ floatx4 shared[];
+    f16x8* planes = reinterpret_cast<f16x8*>(shared);                   // [turn][half][BLOCK]
+    float* factors = reinterpret_cast<float*>(planes + 4 * BLOCK);      // [turn][half][NT * 16]
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = wave >> 2;
+    const uint32_t tile = (blockIdx.x * 4 + (wave & 3)) * RT;
+    const uint32_t first = blockIdx.y * a.per;
+    const uint32_t end = first + a.per < a.p.blocks ? first + a.per : a.p.blocks;
+    const uint32_t chunk = threadIdx.x & 15, row = (threadIdx.x >> 4) & 15;
+    float v[NT][8];
+    bool used[NT];
+    auto load_x = [&](uint32_t block) __attribute__((always_inline)) {
+        const uint32_t col = (block + half) * 128 + chunk * 8;
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const uint32_t token = n * 16 + row;
+            const bool real = token < a.tokens && block + half < end && col < a.p.cols;
+            load_chunk(a.x + (real ? token * a.x_stride + col : 0), v[n]);
+            used[n] = real;
+        }
+    };
+    auto make = [&](uint32_t turn) __attribute__((always_inline)) {
+        f16x8* to = planes + (turn * 2 + half) * BLOCK + (chunk >> 2) * 128 + (chunk & 3) * 16 +
+            ((row + (chunk & 3) + 4 * (chunk >> 2)) & 15);
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            f16x8 hi, lo;
+            const float back = chunk_planes(v[n], used[n], hi, lo);
+            to[n * 512] = hi;
+            to[n * 512 + 64] = lo;
+            if (chunk == 0) {
+                factors[(turn * 2 + half) * NT * 16 + n * 16 + row] = back;
+            }
+        }
+    };
+    floatx4 acc[RT][NT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            acc[t][n] = (floatx4){0, 0, 0, 0};
+        }
+    }
+    const NibbleMasks mask;
+    // Loads are unconditional, as in k_q4_few: blocks past the end are the last one again.
+    auto ask = [&](Q4Block<PER, RT>& to, uint32_t block) __attribute__((always_inline)) {
+        to.load(a, tile, block + half < end ? block + half : end - 1, lane);
+    };
+    load_x(first);
+    Q4Block<PER, RT> ring[2];
+    __builtin_amdgcn_sched_barrier(0);   // in their order, which the waits go by
+    ask(ring[0], first);
+    __builtin_amdgcn_sched_barrier(0);
+    ask(ring[1], first + 2);
+    __builtin_amdgcn_sched_barrier(0);
+    make(0);
+    for (uint32_t b = first; b < end; b += 4) {
+#pragma unroll
+        for (int d = 0; d < 2; d++) {
+            const uint32_t at = b + 2 * d;
+            if (at >= end) {
+                break;
+            }
+            // Planes of this turn are there and the other turn's are done with; codes on
+            // their way go on.
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+            load_x(at + 2);
+            if (at + half < end) {
+                const f16x8* from = planes + (d * 2 + half) * BLOCK + g * 16;
+                auto x = [&](int n, int j, int plane) __attribute__((always_inline)) {
+                    return from[n * 512 + j * 128 + plane * 64 + ((lane + g + 4 * j) & 15)];
+                };
+                float f[NT];
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    f[n] = factors[(d * 2 + half) * NT * 16 + n * 16 + (lane & 15)];
+                }
+                q4_multiply_block<PER, RT, NT>(ring[d], x, f, acc, mask);
+            }
+            __builtin_amdgcn_sched_barrier(0);   // as in k_q4_few
+            ask(ring[d], at + 4);
+            make(1 - d);
+        }
+    }
+    // The second half's sums join the first's.
+    __syncthreads();
+    floatx4* joined = shared + (wave & 3) * RT * NT * 64 + lane;
+    if (half == 1) {
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                joined[(t * NT + n) * 64] = acc[t][n];
+            }
+        }
+    }
+    __syncthreads();
+    if (half == 1) {
+        return;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const uint32_t token = n * 16 + (lane & 15);
+        if (token >= a.tokens) {
+            continue;
+        }
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            if (tile + t < a.p.tiles) {
+                q4_put(a, acc[t][n] + joined[(t * NT + n) * 64], token, (tile + t) * 16 + 4 * g,
+                    blockIdx.y, gridDim.y);
+            }
+        }
+    }
 }
 
 // More tokens: planes made once, by one workgroup a token. A thread holds its first
@@ -429,15 +665,15 @@ k_q4_planes(Q4Args a, f16x8* planes, float* factors)
     }
 }
 
-// Four waves with two row tiles each share the planes of NT token tiles in LDS, which
+// Four waves with two row tiles each share the planes of four token tiles in LDS, which
 // is filled a block ahead by loads straight into it; codes come a block ahead too.
-// grid (8-tile row groups, token tiles / NT, column splits). Planes of tokens past the
+// grid (8-tile row groups, token tiles / 4, column splits). Planes of tokens past the
 // last hold anything: a column's sums are its own and these are not stored.
-template <int PER, int NT>
+template <int PER>
 __global__ void __launch_bounds__(256)
 k_q4_many(Q4Args a)
 {
-    constexpr int RT = 2, BLOCK = NT * 512;   // f16x8 of a block's planes
+    constexpr int RT = 2, NT = 4, BLOCK = NT * 512;   // f16x8 of a block's planes
     __shared__ f16x8 shared[2][BLOCK];
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -507,19 +743,7 @@ k_q4_many(Q4Args a)
             for (int i = 0; i < 4; i++) {
                 v[i] *= factor;
             }
-            if (gridDim.z > 1) {
-                const size_t width = (size_t)a.p.tiles * 16;
-                *reinterpret_cast<floatx4*>(a.part +
-                    ((size_t)blockIdx.z * a.tokens + token) * width + row) = v;
-                continue;
-            }
-            float* y = a.y + token * a.y_stride + row;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if (row + e < a.p.rows) {
-                    y[e] = v[e];
-                }
-            }
+            q4_put(a, v, token, row, blockIdx.z, gridDim.z);
         }
     }
 }
@@ -562,18 +786,24 @@ extern "C" int lh_launch_q4_quantize(const float* w, uint32_t rows, uint32_t col
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
-// How a product runs. few: planes in the kernel itself, rt row tiles a workgroup.
-// Otherwise nt token tiles a workgroup and `splits` column splits, with scratch for
-// planes, factors and parts.
+// How a product runs: few tokens, up to SOME_TOKENS, or more. rt row tiles a workgroup of
+// k_q4_few, of which there are `groups`; otherwise nt token tiles a workgroup and `splits`
+// column splits, with scratch for their parts and, past SOME_TOKENS, planes and factors.
+enum Q4Way { Q4_FEW, Q4_SOME, Q4_MANY };
 struct Q4Plan {
-    bool few;
-    uint32_t nt, rt, splits, per;
+    Q4Way way;
+    uint32_t nt, rt, groups, splits, per;
     size_t planes, factors;   // bytes
 };
 
-// Workgroups to aim for, one a unit (down of 45 tokens: 21 us with 256, 25 with 128,
-// 24 with 384); the row tiles of a k_q4_many workgroup.
-enum { Q4_WORKGROUPS = 256, MANY_TILES = 8 };
+// The row tiles of a k_q4_some or k_q4_many workgroup; the most tokens of the first
+// (64 tokens, 3072 x 4096: 16.7 us against k_q4_many's 19.8; its planes are made again
+// for every 8 row tiles, past 64 tokens for every 64 tokens too).
+// START and JOIN: what a workgroup's start and the launch that joins splits cost, in
+// blocks (18432 x 3072, 45 and 64 tokens: 35.8 and 40.9 us with 3 and 3, which splits,
+// 38.0 and 44.2 with 6 and 6, which does not).
+enum { MANY_TILES = 8, SOME_TOKENS = 64, START = 3, JOIN = 3 };
+
 
 static Q4Plan q4_plan(uint32_t rows, uint32_t cols, uint32_t tokens)
 {
@@ -581,40 +811,71 @@ static Q4Plan q4_plan(uint32_t rows, uint32_t cols, uint32_t tokens)
     Q4Plan p = {};
     p.per = (blocks + WAVES - 1) / WAVES;
     p.splits = 1;
-    p.few = tokens <= 16 && tokens * p.per <= STAGED;
-    if (p.few) {
-        // Row tiles of a workgroup: one round of workgroups, two on a unit where their
-        // LDS fits twice.
-        const uint32_t units = q4_few_lds(tokens, p.per, 1) > 80 * 1024 ? 256 : 512;
-        const uint32_t rt = (tiles + units - 1) / units;
-        p.rt = rt < 6 ? rt : 6;
+    if (tokens <= 16 && tokens * p.per <= STAGED) {
+        p.way = Q4_FEW;
+        // Two row tiles use an operand twice, which pays once a workgroup has many turns
+        // (8 tokens, 131072 rows of 3072: 54 us against 58; 18432 rows: 14 both; 4 tokens,
+        // 3072 rows of 4096: 5.6 with one, 6.7 with two), where their sums fit beside the planes.
+        p.rt = tiles > 2048 && tokens * p.per <= 24 ? 2 : 1;
+        // One round of workgroups, two on a unit where their LDS fits twice, with as many
+        // turns each.
+        const uint32_t units = q4_few_lds(tokens, p.per, p.rt) > 80 * 1024 ? 256 : 512;
+        const uint32_t groups = (tiles + p.rt - 1) / p.rt, turns = (groups + units - 1) / units;
+        p.groups = (groups + turns - 1) / turns;
         return p;
     }
+    p.way = tokens <= SOME_TOKENS ? Q4_SOME : Q4_MANY;
     const uint32_t tt = (tokens + 15) / 16;
     p.nt = tt < 4 ? tt : 4;
     const uint32_t groups = (tiles + MANY_TILES - 1) / MANY_TILES * ((tt + p.nt - 1) / p.nt);
-    uint32_t splits = (Q4_WORKGROUPS + groups - 1) / groups;
+    // Workgroups that run at once: k_q4_some's planes take 33 KiB a token tile.
+    const uint32_t slots = p.way == Q4_SOME && p.nt > 2 ? 256 : 512;
+    uint32_t best = ~0u;
     const uint32_t most = (blocks + 3) / 4;   // four blocks at least
-    splits = splits < most ? splits : most;
-    p.per = (blocks + splits - 1) / splits;
+    for (uint32_t i = 1; i <= most && (i == 1 || groups * i <= 512); i++) {
+        const uint32_t per = (blocks + i - 1) / i;
+        const uint32_t cost = (groups * i + slots - 1) / slots * (per + START) + (i > 1 ? JOIN : 0);
+        if (cost < best) {
+            best = cost;
+            p.per = per;
+        }
+    }
     p.splits = (blocks + p.per - 1) / p.per;
-    p.planes = (size_t)tt * blocks * 8192;
-    p.factors = lh_round16((size_t)tokens * 4);
+    if (p.way == Q4_MANY) {
+        p.planes = (size_t)tt * blocks * 8192;
+        p.factors = lh_round16((size_t)tokens * 4);
+    }
     return p;
 }
 
 template <int PER>
 static void q4_few(const Q4Plan& p, const Q4Args& a, hipStream_t s)
 {
-    const dim3 grid((a.p.tiles + p.rt - 1) / p.rt), block(64 * WAVES);
+    const dim3 grid(p.groups), block(64 * WAVES);
     const size_t lds = q4_few_lds(a.tokens, p.per, p.rt);
-    switch (p.rt) {
-    case 1: hipLaunchKernelGGL((k_q4_few<PER, 1>), grid, block, lds, s, a); break;
-    case 2: hipLaunchKernelGGL((k_q4_few<PER, 2>), grid, block, lds, s, a); break;
-    case 3: hipLaunchKernelGGL((k_q4_few<PER, 3>), grid, block, lds, s, a); break;
-    case 4: hipLaunchKernelGGL((k_q4_few<PER, 4>), grid, block, lds, s, a); break;
-    case 5: hipLaunchKernelGGL((k_q4_few<PER, 5>), grid, block, lds, s, a); break;
-    default: hipLaunchKernelGGL((k_q4_few<PER, 6>), grid, block, lds, s, a); break;
+    if (p.rt == 1) {
+        hipLaunchKernelGGL((k_q4_few<PER, 1, 4>), grid, block, lds, s, a);
+    } else {
+        hipLaunchKernelGGL((k_q4_few<PER, 2, 2>), grid, block, lds, s, a);
+    }
+}
+
+template <int PER, int NT>
+static void q4_some_of(const Q4Plan& p, const Q4Args& a, hipStream_t s)
+{
+    const size_t lds = (size_t)4 * NT * (8192 + 64);
+    hipLaunchKernelGGL((k_q4_some<PER, NT>), dim3((a.p.tiles + MANY_TILES - 1) / MANY_TILES,
+        p.splits), dim3(512), lds, s, a);
+}
+
+template <int PER>
+static void q4_some(const Q4Plan& p, const Q4Args& a, hipStream_t s)
+{
+    switch (p.nt) {
+    case 1: q4_some_of<PER, 1>(p, a, s); break;
+    case 2: q4_some_of<PER, 2>(p, a, s); break;
+    case 3: q4_some_of<PER, 3>(p, a, s); break;
+    default: q4_some_of<PER, 4>(p, a, s); break;
     }
 }
 
@@ -624,21 +885,16 @@ static void q4_many(const Q4Plan& p, const Q4Args& a, hipStream_t s)
     const uint32_t tt = (a.tokens + 15) / 16;
     const dim3 grid((a.p.tiles + MANY_TILES - 1) / MANY_TILES, (tt + p.nt - 1) / p.nt, p.splits);
     const dim3 block(256);
-    switch (p.nt) {
-    case 1: hipLaunchKernelGGL((k_q4_many<PER, 1>), grid, block, 0, s, a); break;
-    case 2: hipLaunchKernelGGL((k_q4_many<PER, 2>), grid, block, 0, s, a); break;
-    case 3: hipLaunchKernelGGL((k_q4_many<PER, 3>), grid, block, 0, s, a); break;
-    default: hipLaunchKernelGGL((k_q4_many<PER, 4>), grid, block, 0, s, a); break;
-    }
+    hipLaunchKernelGGL((k_q4_many<PER>), grid, block, 0, s, a);
 }
 
 template <int PER>
 static void q4_product(const Q4Plan& p, const Q4Args& a, hipStream_t s)
 {
-    if (p.few) {
-        q4_few<PER>(p, a, s);
-    } else {
-        q4_many<PER>(p, a, s);
+    switch (p.way) {
+    case Q4_FEW: q4_few<PER>(p, a, s); break;
+    case Q4_SOME: q4_some<PER>(p, a, s); break;
+    default: q4_many<PER>(p, a, s); break;
     }
 }
 
@@ -648,7 +904,7 @@ static void q4_product(const Q4Plan& p, const Q4Args& a, hipStream_t s)
 extern "C" size_t lh_q4_scratch_bytes(uint32_t cols, uint32_t tokens)
 {
     const Q4Plan p = q4_plan(1, cols, tokens);
-    if (p.few) {
+    if (p.way == Q4_FEW) {
         return 0;
     }
     const size_t parts = cols > 128 * 4 ? (size_t)512 * MANY_TILES * 16 * 4 : 0;
@@ -664,7 +920,7 @@ extern "C" int lh_launch_q4_matvec(const uint8_t* packed, const float* x, size_t
     float* factors = reinterpret_cast<float*>(scratch + p.planes);
     const Q4Args a = {packed, q4_shape(rows, cols, group), x, y, x_stride, y_stride, tokens, p.per,
         planes, factors, reinterpret_cast<float*>(scratch + p.planes + p.factors)};
-    if (!p.few) {
+    if (p.way == Q4_MANY) {
         hipLaunchKernelGGL(k_q4_planes, dim3(tokens), dim3(1024), 0, s, a, planes, factors);
         if (hipGetLastError() != hipSuccess) {
             return -1;
