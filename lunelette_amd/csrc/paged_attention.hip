@@ -505,6 +505,9 @@ k_paged_prompt(AttentionArgs a)
         }
         for (int32_t b = first; b < end; b++) {
             SharedBlock<D, Q4>&now = blocks[(b - first) & 1], &other = blocks[(b - first + 1) & 1];
+            if (!Q4) {
+                __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's part of the block
+            }
             __syncthreads();   // this block is there, the other buffer is free
             if (b + 1 < end) {
                 if constexpr (Q4) {

@@ -707,6 +707,7 @@ k_q4_many(Q4Args a)
     stage(first, shared[0]);
     for (uint32_t b = first; b < end; b++) {
         Q4Block<PER, RT> next = now;
+        __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's part of the planes
         __syncthreads();   // this block's planes are there, the other buffer is free
         if (b + 1 < end) {
             next.load(a, tile, b + 1, lane);

@@ -43,6 +43,35 @@ def test_q4_matvec(gpu, rows, cols, group, tokens):
     assert np.array_equal(again.view(np.uint32), got.view(np.uint32))
 
 
+@pytest.mark.parametrize("rows,cols,group,tokens", [
+    (33000, 128, 32, 1), (33000, 128, 64, 3), (33003, 384, 128, 7), (9000, 384, 64, 16),
+    (4100, 640, 128, 10), (2000, 2048, 32, 24), (2000, 2080, 32, 48), (777, 5120, 128, 64),
+    (300, 8192, 32, 64), (16, 4160, 64, 31), (600, 4096, 128, 8), (600, 4096, 128, 9)])
+def test_q4_matvec_turns_and_splits(gpu, rows, cols, group, tokens):
+    """Workgroups with several turns of row tiles, tokens to either side of each
+    way to run a product, column splits of odd lengths."""
+    rng = np.random.default_rng(rows + tokens)
+    codes, scales = so.q4_random(rng, rows, cols, group)
+    x = rng.normal(size=(tokens, cols)).astype(np.float32)
+    w = so.q4_weights(codes, scales, group)
+    packed = so.q4_on_device(gpu, codes, scales, group)
+    got = so.q4_run(gpu, packed, x, rows, cols, group, x_pad=1, y_pad=2)
+    close(got, x.astype(np.float64) @ w.T, so.q4_bound(w, x))
+
+
+@pytest.mark.parametrize("tokens", [2, 30, 70])
+def test_q4_matvec_ties(gpu, tokens):
+    """x halfway between two FP16 values: the second plane has the rest."""
+    rows, cols, group = 32, 640, 32
+    rng = np.random.default_rng(tokens)
+    codes, scales = so.q4_random(rng, rows, cols, group)
+    x = (1 + (2 * rng.integers(0, 1024, size=(tokens, cols)) + 1) * 2.0 ** -11).astype(np.float32)
+    x *= rng.choice([-1, 1], size=x.shape)
+    w = so.q4_weights(codes, scales, group)
+    got = so.q4_run(gpu, so.q4_on_device(gpu, codes, scales, group), x, rows, cols, group)
+    close(got, x.astype(np.float64) @ w.T, so.q4_bound(w, x))
+
+
 @pytest.mark.parametrize("tokens", [6, 40])
 def test_q4_matvec_ranges_and_special_rows(gpu, tokens):
     """Rows of every magnitude, a zero row, and rows with an Inf or NaN, which
@@ -425,6 +454,69 @@ def test_paged_special_vectors(gpu, kind):
         want, off = so.attention(q[t], keys, values, t, 0.125)
         close(got[t], want, off)
     assert np.isnan(got[41:]).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,heads,count", [
+    (128, 1, 3), (64, 1, 4), (128, 1, 5), (64, 2, 4), (128, 3, 3), (64, 1, 16), (128, 1, 17),
+    (64, 4, 8), (128, 1, 32), (128, 3, 11), (64, 1, 129), (128, 1, 129)])
+def test_paged_row_tiles(gpu, kind, dim, heads, count):
+    """To either side of every number of rows in a tile, after a prefix; the last
+    position, which only the last token sees, has an Inf among its values."""
+    prefix = 75
+    rng = np.random.default_rng(dim + heads + count)
+    n = prefix + count
+    seq = so.Sequences(gpu, kind, dim, heads, 1, 32, [n], rng)
+    k, v = (rng.normal(size=(n, 1, dim)).astype(np.float32) for _ in range(2))
+    v[n - 1, 0, 5] = np.inf
+    seq.append(seq.batch([n], [n]), k, v)
+    held_k, held_v = so.cache_values(k, kind), so.cache_values(v, kind)
+    q = rng.normal(size=(count, heads, dim)).astype(np.float32)
+    got = seq.attention(seq.batch([count], [n]), q, 0.125)
+    for t in range(count - 1):
+        want, off = so.attention(q[t], held_k[:n - 1], held_v[:n - 1], prefix + t, 0.125)
+        close(got[t], want, off)
+    if kind == lh.CACHE_Q4:
+        assert np.isnan(got[-1]).all()
+        return
+    held_v[n - 1, 0, 5] = 0
+    want, off = so.attention(q[-1], held_k, held_v, n - 1, 0.125)
+    want[:, 5] = np.nan
+    close(got[-1], want, off)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_paged_prompts_from_the_start(gpu, kind, dim):
+    """Prompts at position 0, one query head a KV head: the rows of a tile end in
+    different blocks."""
+    run = Run(gpu, kind, dim, 2, 2, 64, [200, 129, 90], dim)
+    batch, q, _ = run.step([200, 129, 90])
+    got = run.check_attention(batch, q, [200, 129, 90])
+    for _ in range(5):
+        again = run.seq.attention(batch, q, float(np.float32(1 / np.sqrt(dim))))
+        assert np.array_equal(again.view(np.uint32), got.view(np.uint32))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("count", [3, 40])
+@pytest.mark.parametrize("size,scale", [(1e-30, 1e-9), (1e30, 1e-31), (0.0, 1.0), (1e-6, 1e6),
+                                        (100.0, 3.0)])
+def test_paged_query_sizes(gpu, kind, count, size, scale):
+    """Queries and scales whose product alone is of a common size, or vanishes,
+    and scores that leave one position."""
+    rng = np.random.default_rng(count)
+    n, dim = 100, 128
+    seq = so.Sequences(gpu, kind, dim, 2, 1, 64, [n], rng)
+    k, v = (rng.normal(size=(n, 1, dim)).astype(np.float32) for _ in range(2))
+    seq.append(seq.batch([n], [n]), k, v)
+    held_k, held_v = so.cache_values(k, kind), so.cache_values(v, kind)
+    q = (rng.normal(size=(count, 2, dim)) * size).astype(np.float32)
+    scale = float(np.float32(scale))
+    got = seq.attention(seq.batch([count], [n]), q, scale)
+    for t in range(count):
+        want, off = so.attention(q[t], held_k, held_v, n - count + t, scale)
+        close(got[t], want, off)
 
 
 def test_paged_large_offsets(gpu):
