@@ -45,7 +45,8 @@ size_t lh_q4_scratch(size_t cols, size_t tokens);
  * x_stride and y_stride elements apart (x_stride >= cols, y_stride >= rows).
  * Products are formed from x as two FP16 planes scaled by a power of two per
  * token, or per token and 128 columns (each x to 2^-22 of itself or 2^-38 of
- * its row's largest), sums are FP32. A row of x with an Inf or NaN gives NaN in its row of y. */
+ * its row's largest), sums are FP32. A row of x with an Inf or NaN gives NaN in
+ * its row of y. y must not overlap x. */
 int lh_q4_matvec(const void *d_packed, const float *d_x, size_t x_stride, float *d_y,
     size_t y_stride, size_t rows, size_t cols, size_t group, size_t tokens, void *d_scratch,
     size_t scratch_bytes, void *stream);
@@ -76,7 +77,7 @@ int lh_logprobs(const float *d_logits, size_t stride, size_t rows, size_t vocab,
 /* ---- paged KV cache ---- */
 
 enum {
-    LH_CACHE_F16 = 0, /* rows rounded to FP16 */
+    LH_CACHE_F16 = 0, /* rows rounded to FP16 (from 65520 on Inf) */
     /* per (position, KV head) vector of keys or values 4-bit codes and a BF16
      * scale and zero: zero = bf16(min), scale = bf16((max - zero) / 15),
      * code = rint((v - zero) / scale) within 0..15, value = scale * code + zero.
@@ -117,11 +118,14 @@ typedef struct {
  * the rows of their positions in d_cos, d_sin [positions][head_dim] (as
  * lh_yarn writes them: split halves, both halves of a row alike), and writes
  * the rotated queries, times d_qfactor[position] where that is not NULL, to
- * d_q_out (which may be d_q with the same stride). heads is a multiple of kv_heads up to 64 of them
- * each; 0 leaves the queries out. d_cos and d_sin NULL: rotated already. The
- * rotation is formed in 64 bits and rounded once. A token whose position is
- * negative or not below `positions` is not appended, its query row is NaN.
- * Sequences of one call must not append to the same page. */
+ * d_q_out (which may be d_q with the same stride, and overlaps no other tensor).
+ * heads is a multiple of kv_heads up to 64 of them each; 0 leaves the queries
+ * out. d_cos and d_sin NULL: rotated already. The rotation is formed in 64 bits
+ * and rounded to FP32 (for 4-bit codes not at all) before the cache's format.
+ * With d_cos or d_qfactor a token whose position is negative or not below
+ * `positions` is not appended and its query row is NaN; without them that holds
+ * for negative positions. A page that a call appends to must stand in one place
+ * of one sequence's table. */
 int lh_paged_append(const lh_paged_cache *cache, const lh_paged_batch *batch, uint32_t heads,
     const float *d_q, size_t q_stride, const float *d_k, size_t k_stride, const float *d_v,
     size_t v_stride, const float *d_cos, const float *d_sin, uint32_t positions,
@@ -138,8 +142,11 @@ size_t lh_paged_attention_scratch(const lh_paged_cache *cache, const lh_paged_ba
  * KV head h / (heads / kv_heads), scores times scale (positive and finite),
  * into d_out (which must not overlap d_q). A token at a negative position sees
  * nothing and gives 0; one that sees a position without a place in the cache
- * gives NaN. Products are formed from FP16 planes of 22 bits or more, sums and the
- * softmax in FP32. */
+ * gives NaN, as does one that sees a key with an Inf or NaN, or a value with one
+ * (in FP16 pages in that element alone). What no token sees may hold anything.
+ * Products are formed from queries (and probabilities, times the values' scales)
+ * as two FP16 planes, which keep them to 2^-22 of themselves or 2^-38 of the
+ * largest; sums and the softmax are FP32. */
 int lh_paged_attention(const lh_paged_cache *cache, const lh_paged_batch *batch, uint32_t heads,
     const float *d_q, size_t q_stride, float scale, float *d_out, size_t out_stride,
     void *d_scratch, size_t scratch_bytes, void *stream);

@@ -27,10 +27,11 @@ static int aligned(const void *ptr, uintptr_t bytes)
     return ((uintptr_t)ptr & (bytes - 1)) == 0;
 }
 
-/* Row strides stay below 2^40 elements, so no row offset passes 64 bits. */
+/* Row strides stay below 2^36 elements (256 GiB), so no offset of 2^24 rows passes
+ * 64 bits. */
 static int stride_ok(size_t stride, size_t width)
 {
-    return stride >= width && stride <= ((size_t)1 << 40);
+    return stride >= width && stride <= ((size_t)1 << 36);
 }
 
 /* ---- 4-bit weights ---- */
@@ -97,6 +98,9 @@ int lh_q4_matvec(const void *d_packed, const float *d_x, size_t x_stride, float 
     if (need && (!d_scratch || scratch_bytes < need || !aligned(d_scratch, 16))) {
         lh_set_error("q4_matvec: needs %zu bytes of scratch on a 16-byte boundary", need);
         return -1;
+    }
+    if ((const void *)d_x == (const void *)d_y) {
+        return refuse("q4_matvec: y must not overlap x");
     }
     return launched(lh_launch_q4_matvec(d_packed, d_x, x_stride, d_y, y_stride, (uint32_t)rows,
         (uint32_t)cols, (uint32_t)group, (uint32_t)tokens, d_scratch, (hipStream_t)stream),

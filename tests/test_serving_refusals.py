@@ -128,6 +128,13 @@ BAD_Q4 = [(0, 256, 64), (2 ** 20 + 1, 256, 64), (100, 0, 64), (100, 65536 + 64, 
           (100, 250, 64), (100, 256, 16), (100, 256, 0), (100, 96, 64)]
 
 
+def test_q4_refuses_its_own_input(product):
+    assert q4(product, y=P) == -1
+    assert "overlap" in lh.last_error()
+    assert q4(product, xs=2 ** 36 + 1) == -1
+    assert "stride" in lh.last_error()
+
+
 def test_q4_refusals(product):
     for rows, cols, group in BAD_Q4:
         assert product.lh_q4_bytes(rows, cols, group) == 0
