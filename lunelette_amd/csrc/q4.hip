@@ -208,16 +208,30 @@ __device__ __forceinline__ void q4_multiply_block(const Q4Block<PER, RT>& b, con
         for (int t = 0; t < RT; t++) {
             w[t] = codes_minus8(b.w[t][j], mask);
         }
+        // Products that need one another stand four apart where there are as many.
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const f16x8 high = x(n, j, 0), low = x(n, j, 1);
+        for (int n0 = 0; n0 < NT; n0 += 2) {
+            constexpr int TWO = NT > 1 ? 2 : 1;
+            f16x8 at[TWO][2];
 #pragma unroll
-            for (int t = 0; t < RT; t++) {
-                if (j % STEPS == 0) {
-                    d[t][n] = (floatx4){0, 0, 0, 0};
+            for (int i = 0; i < TWO && n0 + i < NT; i++) {
+                at[i][0] = x(n0 + i, j, 0);
+                at[i][1] = x(n0 + i, j, 1);
+            }
+#pragma unroll
+            for (int plane = 0; plane < 2; plane++) {
+#pragma unroll
+                for (int i = 0; i < TWO && n0 + i < NT; i++) {
+#pragma unroll
+                    for (int t = 0; t < RT; t++) {
+                        floatx4& to = d[t][n0 + i];
+                        if (j % STEPS == 0 && plane == 0) {
+                            to = (floatx4){0, 0, 0, 0};
+                        }
+                        to = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[t], at[i][plane], to, 0, 0,
+                            0);
+                    }
                 }
-                d[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[t], high, d[t][n], 0, 0, 0);
-                d[t][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[t], low, d[t][n], 0, 0, 0);
             }
         }
         if (j % STEPS != STEPS - 1) {
@@ -277,16 +291,19 @@ __device__ __forceinline__ void load_chunk(const float* x, float (&v)[8])
 // side have those of a block; its power of two back.
 __device__ __forceinline__ float chunk_planes(float (&v)[8], bool used, f16x8& hi, f16x8& lo)
 {
+    if (!__all(used)) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        v[e] = used ? v[e] : 0.0f;
+        for (int e = 0; e < 8; e++) {
+            v[e] = used ? v[e] : 0.0f;
+        }
     }
-    uint32_t m = 0;   // magnitudes order as their bits; an Inf or NaN is the largest
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const uint32_t bits = __float_as_uint(v[e]) & 0x7fffffffu;
-        m = m > bits ? m : bits;
-    }
+    // A NaN takes no part and stays one in its plane.
+    float f;
+    asm("v_max3_f32 %0, |%1|, |%2|, |%3|" : "=v"(f) : "v"(v[0]), "v"(v[1]), "v"(v[2]));
+    asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(f) : "v"(v[3]), "v"(v[4]));
+    asm("v_max3_f32 %0, %0, |%1|, |%2|" : "+v"(f) : "v"(v[5]), "v"(v[6]));
+    asm("v_max_f32 %0, %0, |%1|" : "+v"(f) : "v"(v[7]));
+    uint32_t m = __float_as_uint(f);   // magnitudes order as their bits
     uint32_t o;   // the row's other lanes by rotations of 8, 4, 2 and 1
     o = (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x128, 0xf, 0xf, false), m = m > o ? m : o;
     o = (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x124, 0xf, 0xf, false), m = m > o ? m : o;
@@ -464,7 +481,7 @@ k_q4_few(Q4Args a)
 // splits). Token t of step j's g is at place (t + g + 4 j) % 16 of its sixteen, so that
 // a token's sixteen chunks go to different banks.
 template <int PER, int NT>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(512, NT == 1 ? 4 : 2)
 k_q4_some(Q4Args a)
 {
     constexpr int RT = 2, BLOCK = NT * 512;   // f16x8 of a block's planes
