@@ -118,7 +118,8 @@ typedef struct {
  * the rows of their positions in d_cos, d_sin [positions][head_dim] (as
  * lh_yarn writes them: split halves, both halves of a row alike), and writes
  * the rotated queries, times d_qfactor[position] where that is not NULL, to
- * d_q_out (which may be d_q with the same stride, and overlaps no other tensor).
+ * d_q_out (which may be d_q with the same stride, and otherwise shares no element
+ * with another tensor).
  * heads is a multiple of kv_heads up to 64 of them each; 0 leaves the queries
  * out. d_cos and d_sin NULL: rotated already. The rotation is formed in 64 bits
  * and rounded to FP32 (for 4-bit codes not at all) before the cache's format.
