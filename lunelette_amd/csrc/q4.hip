@@ -109,8 +109,8 @@ k_q4_quantize(const float* __restrict__ w, Q4Shape p, uint8_t* __restrict__ pack
 // The product. A wave takes 128-column blocks of RT row tiles for NT tiles of 16
 // tokens: y^T tile [16 rows][16 tokens] = W X^T by 16x16x32 FP16 matrix instructions,
 // W the codes minus 8 (exact), X two planes h + l of x times a power of two: 22 bits of
-// the largest x that shares the power (of a token's 128 columns; all of its columns past
-// SOME_TOKENS). A group's sums are formed from 0 and join the row's by its scale in FP32,
+// the largest x that shares the power (of a token's 128 columns, in k_q4_many of all of
+// its columns). A group's sums are formed from 0 and join the row's by its scale in FP32,
 // so a scale never rounds a weight. Codes and scales of the blocks to come are on their
 // way while one is multiplied.
 // Bound: the codes' bytes. Measured, cold weights: 131072 x 3072 (214 MB) for one token
@@ -475,10 +475,10 @@ k_q4_few(Q4Args a)
     }
 }
 
-// Up to 64 tokens: eight waves, two row tiles each, in two halves that take every
+// Some tokens: eight waves, two row tiles each, in two halves that take every
 // second block. The blocks' planes are shared in LDS, made for the next two blocks while
 // two are multiplied, with codes two turns ahead. grid (8-tile row groups, column
-// splits). Token t of step j's g is at place (t + g + 4 j) % 16 of its sixteen, so that
+// splits, NT token tiles). Token t of step j's g is at place (t + g + 4 j) % 16 of its sixteen, so that
 // a token's sixteen chunks go to different banks.
 template <int PER, int NT>
 __global__ void __launch_bounds__(512, NT == 1 ? 4 : 2)
@@ -494,13 +494,14 @@ k_q4_some(Q4Args a)
     const uint32_t first = blockIdx.y * a.per;
     const uint32_t end = first + a.per < a.p.blocks ? first + a.per : a.p.blocks;
     const uint32_t chunk = threadIdx.x & 15, row = (threadIdx.x >> 4) & 15;
+    const uint32_t token0 = blockIdx.z * NT * 16;
     float v[NT][8];
     bool used[NT];
     auto load_x = [&](uint32_t block) __attribute__((always_inline)) {
         const uint32_t col = (block + half) * 128 + chunk * 8;
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            const uint32_t token = n * 16 + row;
+            const uint32_t token = token0 + n * 16 + row;
             const bool real = token < a.tokens && block + half < end && col < a.p.cols;
             load_chunk(a.x + (real ? token * a.x_stride + col : 0), v[n]);
             used[n] = real;
@@ -589,7 +590,7 @@ k_q4_some(Q4Args a)
     }
 #pragma unroll
     for (int n = 0; n < NT; n++) {
-        const uint32_t token = n * 16 + (lane & 15);
+        const uint32_t token = token0 + n * 16 + (lane & 15);
         if (token >= a.tokens) {
             continue;
         }
@@ -804,9 +805,9 @@ extern "C" int lh_launch_q4_quantize(const float* w, uint32_t rows, uint32_t col
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
-// How a product runs: few tokens, up to SOME_TOKENS, or more. rt row tiles a workgroup of
+// How a product runs: few tokens, some, or many. rt row tiles a workgroup of
 // k_q4_few, of which there are `groups`; otherwise nt token tiles a workgroup and `splits`
-// column splits, with scratch for their parts and, past SOME_TOKENS, planes and factors.
+// column splits, with scratch for their parts and, past 64 tokens, planes and factors.
 enum Q4Way { Q4_FEW, Q4_SOME, Q4_MANY };
 struct Q4Plan {
     Q4Way way;
@@ -814,14 +815,14 @@ struct Q4Plan {
     size_t planes, factors;   // bytes
 };
 
-// The row tiles of a k_q4_some or k_q4_many workgroup; the most tokens of the first
-// (64 tokens, 3072 x 4096: 16.7 us against k_q4_many's 19.8; its planes are made again
-// for every 8 row tiles, past 64 tokens for every 64 tokens too).
+// The row tiles of a k_q4_some or k_q4_many workgroup. The first makes its planes again
+// for every 8 row tiles and 64 tokens, the second reads those of a launch of its own: the
+// first up to 64 tokens (64 tokens, 3072 x 4096: 16.5 us against 19.8), and up to 128 where
+// there are at most SOME_TILES row tiles (100 tokens: 6144 x 3072 26 us against 28, 18432 x
+// 3072 88 against 68).
 // START and JOIN: what a workgroup's start and the launch that joins splits cost, in
-// blocks (18432 x 3072, 45 and 64 tokens: 35.8 and 40.9 us with 3 and 3, which splits,
-// 38.0 and 44.2 with 6 and 6, which does not).
-enum { MANY_TILES = 8, SOME_TOKENS = 64, START = 3, JOIN = 3 };
-
+// blocks (2 to 8 give the same times).
+enum { MANY_TILES = 8, SOME_TILES = 512, START = 3, JOIN = 3 };
 
 static Q4Plan q4_plan(uint32_t rows, uint32_t cols, uint32_t tokens)
 {
@@ -842,12 +843,13 @@ static Q4Plan q4_plan(uint32_t rows, uint32_t cols, uint32_t tokens)
         p.groups = (groups + turns - 1) / turns;
         return p;
     }
-    p.way = tokens <= SOME_TOKENS ? Q4_SOME : Q4_MANY;
-    const uint32_t tt = (tokens + 15) / 16;
-    p.nt = tt < 4 ? tt : 4;
-    const uint32_t groups = (tiles + MANY_TILES - 1) / MANY_TILES * ((tt + p.nt - 1) / p.nt);
-    // Workgroups that run at once: k_q4_some's planes take 33 KiB a token tile.
-    const uint32_t slots = p.way == Q4_SOME && p.nt > 2 ? 256 : 512;
+    const uint32_t tt = (tokens + 15) / 16, token_groups = (tt + 3) / 4;
+    p.way = token_groups == 1 || (token_groups == 2 && tiles <= SOME_TILES) ? Q4_SOME : Q4_MANY;
+    p.nt = p.way == Q4_SOME ? (tt + token_groups - 1) / token_groups : 4;
+    const uint32_t groups = (tiles + MANY_TILES - 1) / MANY_TILES * token_groups;
+    // Workgroups that run at once: registers leave room for one of k_q4_some's on a unit
+    // past one token tile.
+    const uint32_t slots = p.way == Q4_SOME && p.nt > 1 ? 256 : 512;
     uint32_t best = ~0u;
     const uint32_t most = (blocks + 3) / 4;   // four blocks at least
     for (uint32_t i = 1; i <= most && (i == 1 || groups * i <= 512); i++) {
@@ -859,7 +861,7 @@ static Q4Plan q4_plan(uint32_t rows, uint32_t cols, uint32_t tokens)
         }
     }
     p.splits = (blocks + p.per - 1) / p.per;
-    if (p.way == Q4_MANY) {
+    if (token_groups > 1) {   // (whatever the rows are: scratch is sized without them)
         p.planes = (size_t)tt * blocks * 8192;
         p.factors = lh_round16((size_t)tokens * 4);
     }
@@ -883,7 +885,7 @@ static void q4_some_of(const Q4Plan& p, const Q4Args& a, hipStream_t s)
 {
     const size_t lds = (size_t)4 * NT * (8192 + 64);
     hipLaunchKernelGGL((k_q4_some<PER, NT>), dim3((a.p.tiles + MANY_TILES - 1) / MANY_TILES,
-        p.splits), dim3(512), lds, s, a);
+        p.splits, (a.tokens + NT * 16 - 1) / (NT * 16)), dim3(512), lds, s, a);
 }
 
 template <int PER>
@@ -916,9 +918,9 @@ static void q4_product(const Q4Plan& p, const Q4Args& a, hipStream_t s)
     }
 }
 
-// For any number of rows: splits appear below 256 workgroups and bring them to less
-// than 512, of eight row tiles and (past 64 tokens more workgroups, not more tokens)
-// 64 tokens, so their parts hold at most 512 * 8 * 16 rows of min(tokens, 64).
+// For any number of rows: with column splits there are at most 512 workgroups, of eight
+// row tiles and (past 64 tokens more workgroups, not more tokens) 64 tokens, so their
+// parts hold at most 512 * 8 * 16 rows of min(tokens, 64).
 extern "C" size_t lh_q4_scratch_bytes(uint32_t cols, uint32_t tokens)
 {
     const Q4Plan p = q4_plan(1, cols, tokens);

@@ -59,6 +59,20 @@ def test_q4_matvec_turns_and_splits(gpu, rows, cols, group, tokens):
     close(got, x.astype(np.float64) @ w.T, so.q4_bound(w, x))
 
 
+@pytest.mark.parametrize("rows,tokens", [(1000, 65), (1000, 96), (1000, 97), (1000, 128),
+                                         (1000, 129), (8192, 80), (8193, 80), (8, 128)])
+def test_q4_matvec_two_token_groups(gpu, rows, tokens):
+    """Past 64 tokens, to either side of where a launch of its own makes the planes."""
+    cols, group = 1056, 32
+    rng = np.random.default_rng(rows + tokens)
+    codes, scales = so.q4_random(rng, rows, cols, group)
+    x = rng.normal(size=(tokens, cols)).astype(np.float32)
+    w = so.q4_weights(codes, scales, group)
+    packed = so.q4_on_device(gpu, codes, scales, group)
+    got = so.q4_run(gpu, packed, x, rows, cols, group, x_pad=2, y_pad=1)
+    close(got, x.astype(np.float64) @ w.T, so.q4_bound(w, x))
+
+
 @pytest.mark.parametrize("tokens", [2, 30, 70])
 def test_q4_matvec_ties(gpu, tokens):
     """x halfway between two FP16 values: the second plane has the rest."""
