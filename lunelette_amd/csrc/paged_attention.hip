@@ -343,15 +343,26 @@ enum { PROMPT_ROWS = 128 };
 // grid (KV heads, sequences, tiles of the splits in turn): the tiles of a KV head of
 // eight share an XCD and its L2. One barrier a block: while a block is multiplied the
 // next one is decoded into the other buffer and the one after is on its way.
+// Of 4-bit pages two teams of four waves take every second block of a split for the same
+// rows and meet in LDS at its end, which halves the parts that splits leave in memory (256
+// tokens after 4096: 57.1 us, with one team and twice the splits 60.6; 64 tokens 32 and
+// 36). FP16 pages wait for the other team's loads too then (57.2 against 53.5).
+template <bool Q4>
+constexpr int TEAMS = Q4 ? 2 : 1;
+
 template <int D, bool Q4>
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__(256 * TEAMS<Q4>, 2)
 k_paged_prompt(AttentionArgs a)
 {
     typedef PageLayout<D, Q4> Layout;
+    constexpr int STEP = TEAMS<Q4>;
     constexpr uint32_t LOADERS = D / 32;   // waves that bring four fragments each
-    __shared__ SharedBlock<D, Q4> blocks[2];
+    __shared__ SharedBlock<D, Q4> buffers[2 * STEP];
+    __shared__ float stats[4][2][2][16];   // of the second team: [wave][column tile][m, sum]
     const uint32_t h = blockIdx.x, s = blockIdx.y, lane = threadIdx.x & 63;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t team = STEP > 1 ? waves >> 2 : 0, wave = STEP > 1 ? waves & 3 : waves;
+    SharedBlock<D, Q4>* blocks = buffers + 2 * team;
     const uint32_t split = blockIdx.z / a.tiles;
     const Span span = batch_span(a.batch, s);
     const int64_t rows = span.count * a.group;
@@ -373,20 +384,20 @@ k_paged_prompt(AttentionArgs a)
         if (split && (int64_t)split * chunk >= steps) {
             continue;   // nothing for this split: the join does not ask for it
         }
-        const int32_t first = 2 * (int32_t)split * chunk;
-        const int32_t end = all - first < 2 * chunk ? all : first + 2 * chunk;
+        const int32_t start = 2 * (int32_t)split * chunk, first = start + (int32_t)team;
+        const int32_t end = all - start < 2 * chunk ? all : start + 2 * chunk;
         PromptRows<D, Q4> c;
         c.lane = lane;
         c.g = lane >> 4;
-        // Lane i has the page ids of blocks first + 64 n + i.
+        // Lane i has the page ids of the team's blocks 64 n + i.
         int32_t ids = 0;
         u32x4 raw;
         uint32_t words = 0;
         bool good = true;
         auto locate = [&](int32_t b, uint32_t& slot) __attribute__((always_inline)) {
-            const int32_t turn = b - first;
+            const int32_t turn = (b - first) / STEP;
             if ((turn & 63) == 0) {
-                const int64_t at = (int64_t)((uint64_t)((uint32_t)b + lane) * a.per_page >> 32);
+                const int64_t at = (int64_t)((uint64_t)((uint32_t)b + STEP * lane) * a.per_page >> 32);
                 ids = at < a.batch.width ? table[at] : -1;
             }
             const uint32_t page = (uint32_t)((uint64_t)(uint32_t)b * a.per_page >> 32);
@@ -499,41 +510,81 @@ k_paged_prompt(AttentionArgs a)
         }
         if (Q4 && first < end) {
             decode(first, blocks[0]);
-            if (first + 1 < end) {
-                ask(first + 1);
+            if (first + STEP < end) {
+                ask(first + STEP);
             }
         }
-        for (int32_t b = first; b < end; b++) {
-            SharedBlock<D, Q4>&now = blocks[(b - first) & 1], &other = blocks[(b - first + 1) & 1];
+        // Both teams pass the same barriers.
+        for (int32_t b = first; b - (int32_t)team < end; b += STEP) {
+            const int32_t turn = (b - first) / STEP & 1;
+            SharedBlock<D, Q4>&now = blocks[turn], &other = blocks[1 - turn];
             if (!Q4) {
                 __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this wave's part of the block
             }
             __syncthreads();   // this block is there, the other buffer is free
-            if (b + 1 < end) {
+            if (b + STEP < end) {
                 if constexpr (Q4) {
-                    decode(b + 1, other);
-                    if (b + 2 < end) {
-                        ask(b + 2);
+                    decode(b + STEP, other);
+                    if (b + 2 * STEP < end) {
+                        ask(b + 2 * STEP);
                     }
                 } else {
-                    fetch(b + 1, other);
+                    fetch(b + STEP, other);
                 }
             }
-            if (32 * b <= c.high) {
+            if (b < end && 32 * b <= c.high) {
                 c.block(now, 32 * b);
             }
+        }
+        // The second team's sums, relative to its own maxima, to the first.
+        if (STEP > 1) {
+            __syncthreads();
+        }
+        floatx4* joined = reinterpret_cast<floatx4*>(buffers) + wave * (D / 8) * 64 + lane;
+        const float back = Q4 ? 1.0f / c.shift : 1.0f / P_SCALE;   // powers of two
+        float sum[2];
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+            sum[n] = c.lost[n] ? __builtin_nanf("") : column_sum(c.sum[n]);
+            const float offset = Q4 ? column_sum(c.offset[n]) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) {
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    c.acc[n][i][r] = __builtin_fmaf(c.acc[n][i][r], back, offset);
+                }
+                if (team) {
+                    joined[(n * (D / 16) + i) * 64] = c.acc[n][i];
+                }
+            }
+            if (team && c.g == 0) {
+                stats[wave][n][0][lane] = c.m[n];
+                stats[wave][n][1][lane] = sum[n];
+            }
+        }
+        if (STEP > 1) {
+            __syncthreads();
+        }
+        if (team) {
+            continue;   // its next tile begins with a barrier, before LDS is written again
         }
         const bool whole = steps <= chunk;   // no other split has a part
 #pragma unroll
         for (int n = 0; n < 2; n++) {
-            const float sum = c.lost[n] ? __builtin_nanf("") : column_sum(c.sum[n]);
-            const float offset = column_sum(c.offset[n]);
             if (tile * PROMPT_ROWS + 32 * wave + 16 * n + (lane & 15) >= rows) {
                 continue;
             }
-            // (Powers of two; no position at all: 0.)
-            const float back = Q4 ? 1.0f / c.shift : 1.0f / P_SCALE;
-            const float over = whole ? sum == 0 ? 0.0f : 1.0f / sum : 1.0f;
+            // A team that saw nothing holds sums of 0, or NaN for a lost position.
+            float m = c.m[n], keep = 1, keep1 = 0, all_sum = sum[n];
+            if (STEP > 1) {
+                const float m1 = stats[wave][n][0][lane & 15];
+                m = fmaxf(m, m1);
+                keep = c.m[n] > -__builtin_inff() ? __builtin_amdgcn_exp2f(c.m[n] - m) : 1.0f;
+                keep1 = m1 > -__builtin_inff() ? __builtin_amdgcn_exp2f(m1 - m) : 1.0f;
+                all_sum = __builtin_fmaf(stats[wave][n][1][lane & 15], keep1, sum[n] * keep);
+            }
+            // (No position at all: 0.)
+            const float over = whole ? all_sum == 0 ? 0.0f : 1.0f / all_sum : 1.0f;
             const int64_t row = row_of(n);
             const size_t token = (size_t)(span.begin + row / a.group);
             const size_t head = (size_t)h * a.group + row % a.group;
@@ -541,16 +592,19 @@ k_paged_prompt(AttentionArgs a)
             float* to = whole ? a.out + token * a.out_stride + head * D : a.part + at * D;
 #pragma unroll
             for (int i = 0; i < D / 16; i++) {
-                float4 v;
-                float* f = &v.x;
+                floatx4 y = c.acc[n][i];
+                if (STEP > 1) {
+                    const floatx4 other = joined[(n * (D / 16) + i) * 64];
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    f[r] = __builtin_fmaf(c.acc[n][i][r], back, Q4 ? offset : 0.0f) * over;
+                    for (int r = 0; r < 4; r++) {
+                        y[r] = __builtin_fmaf(other[r], keep1, y[r] * keep);
+                    }
                 }
+                const float4 v = make_float4(y[0] * over, y[1] * over, y[2] * over, y[3] * over);
                 store4(to + 16 * i + 4 * c.g, v);
             }
             if (!whole && c.g == 0) {
-                a.tops[at] = make_float2(c.m[n], sum);
+                a.tops[at] = make_float2(m, all_sum);
             }
         }
     }
@@ -1197,9 +1251,9 @@ using namespace lh;
 // workgroup's start (32 sequences up to 4352 in FP16: 30 us with 12 or 16, 33 with 24), and about
 // WORKGROUPS in all, so that sequences of other lengths than the bound spread evenly
 // (64 up to 17920 in 4 bits: 102 us with 1024, 103 with 2048, 127 with 512, 122 with 8192).
-// A workgroup of a prompt has 128 rows, and the splits' parts are as large as its output
-// for each: PROMPT_WORKGROUPS in all (256 tokens after 4096 positions: 57 us with 512,
-// 68 with 256, 118 with 128), PROMPT_CHUNK steps at least.
+// A prompt's workgroup (team) has 128 rows, and the splits' parts are as large as its
+// output for each: PROMPT_WORKGROUPS teams in all (256 tokens after 4096 positions, one
+// team a workgroup: 57 us with 512, 68 with 256, 118 with 128), PROMPT_CHUNK steps at least.
 enum { RESIDENT = 512, WORKGROUPS = 2048, MIN_CHUNK = 8, FULL_CHUNK = 16,
     PROMPT_WORKGROUPS = 512, PROMPT_CHUNK = 4 };
 
@@ -1230,7 +1284,8 @@ static AttentionPlan attention_plan(const lh_paged_cache* c, const lh_paged_batc
         chunk = chunk < FULL_CHUNK ? FULL_CHUNK : chunk;
     }
     if (p.tile == PROMPT_ROWS) {
-        chunk = (all + PROMPT_WORKGROUPS - 1) / PROMPT_WORKGROUPS;
+        const uint32_t groups = PROMPT_WORKGROUPS / (c->kind == LH_CACHE_Q4 ? TEAMS<true> : 1);
+        chunk = (all + groups - 1) / groups;
         chunk = chunk < PROMPT_CHUNK ? PROMPT_CHUNK : chunk;
     }
     const uint64_t most = 65535 / p.tiles < SPLITS ? 65535 / p.tiles : SPLITS;
@@ -1260,7 +1315,8 @@ static void attention(const lh_paged_cache* c, const lh_paged_batch* b, const At
     case 4: hipLaunchKernelGGL((k_paged_decode<D, Q4, 4>), grid, block, 0, s, a); break;
     case 8: hipLaunchKernelGGL((k_paged_decode<D, Q4, 8>), grid, block, 0, s, a); break;
     case 16: hipLaunchKernelGGL((k_paged_decode<D, Q4, 16>), grid, block, 0, s, a); break;
-    default: hipLaunchKernelGGL((k_paged_prompt<D, Q4>), grid, block, 0, s, a); break;
+    default: hipLaunchKernelGGL((k_paged_prompt<D, Q4>), grid, dim3(256 * TEAMS<Q4>), 0, s, a);
+        break;
     }
     if (p.splits > 1) {
         const uint32_t query = b->max_query < b->tokens ? b->max_query : b->tokens;
