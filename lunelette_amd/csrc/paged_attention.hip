@@ -397,7 +397,8 @@ k_paged_prompt(AttentionArgs a)
         auto locate = [&](int32_t b, uint32_t& slot) __attribute__((always_inline)) {
             const int32_t turn = (b - first) / STEP;
             if ((turn & 63) == 0) {
-                const int64_t at = (int64_t)((uint64_t)((uint32_t)b + STEP * lane) * a.per_page >> 32);
+                const uint64_t block = (uint32_t)b + STEP * lane;
+                const int64_t at = (int64_t)(block * a.per_page >> 32);
                 ids = at < a.batch.width ? table[at] : -1;
             }
             const uint32_t page = (uint32_t)((uint64_t)(uint32_t)b * a.per_page >> 32);
@@ -467,7 +468,8 @@ k_paged_prompt(AttentionArgs a)
 #pragma unroll
                 for (int w = 0; w < 4; w++) {
                     __builtin_amdgcn_global_load_lds(
-                        (const __attribute__((address_space(1))) void*)(from + 1024 * w + 16 * lane),
+                        (const __attribute__((address_space(1))) void*)(from + 1024 * w +
+                            16 * lane),
                         (__attribute__((address_space(3))) void*)&to.fragment[4 * wave + w][0], 16,
                         0, 0);
                 }
@@ -766,8 +768,8 @@ struct Decode {
 
     // The softmax over the step and the operands of the second product: p (times the
     // value scales) in planes, pairs 0 and 1 of tile PACK * w + u in words 2 w and 2 w + 1.
-    __device__ __forceinline__ void probabilities(const Step& step, float (&p)[C], int32_t base, bool edge,
-        uint32_t (&ph)[C / 2], uint32_t (&pl)[C / 2])
+    __device__ __forceinline__ void probabilities(const Step& step, float (&p)[C], int32_t base,
+        bool edge, uint32_t (&ph)[C / 2], uint32_t (&pl)[C / 2])
     {
         float scale[C], z[C];
         if (Q4) {
@@ -974,8 +976,12 @@ k_paged_decode(AttentionArgs a)
         };
         int32_t x = first + (int32_t)wave;
         DecodeStep<D, Q4, C> step;
-        auto keys = [&](auto& to) __attribute__((always_inline)) { to.load_keys(part, slot, a.cache.page_size, lane); };
-        auto values = [&](auto& to) __attribute__((always_inline)) { to.load_values(part, slot, a.cache.page_size, lane); };
+        auto keys = [&](auto& to) __attribute__((always_inline)) {
+            to.load_keys(part, slot, a.cache.page_size, lane);
+        };
+        auto values = [&](auto& to) __attribute__((always_inline)) {
+            to.load_values(part, slot, a.cache.page_size, lane);
+        };
         if (x < end) {
             locate(x, 0);
             keys(step);

@@ -478,8 +478,10 @@ k_q4_few(Q4Args a)
 // Some tokens: eight waves, two row tiles each, in two halves that take every
 // second block. The blocks' planes are shared in LDS, made for the next two blocks while
 // two are multiplied, with codes two turns ahead. grid (8-tile row groups, column
-// splits, NT token tiles). Token t of step j's g is at place (t + g + 4 j) % 16 of its sixteen, so that
-// a token's sixteen chunks go to different banks.
+// splits, NT token tiles). Token t of step j's g is at place (t + g + 4 j) % 16 of its
+// sixteen, so that a token's sixteen chunks go to different banks.
+// Bound by its vector instructions, half of which make the planes: 45 tokens, 3072 x 9216
+// (14 MB) 14 us and 4 for the join.
 template <int PER, int NT>
 __global__ void __launch_bounds__(512, NT == 1 ? 4 : 2)
 k_q4_some(Q4Args a)
@@ -834,7 +836,8 @@ static Q4Plan q4_plan(uint32_t rows, uint32_t cols, uint32_t tokens)
         p.way = Q4_FEW;
         // Two row tiles use an operand twice, which pays once a workgroup has many turns
         // (8 tokens, 131072 rows of 3072: 54 us against 58; 18432 rows: 14 both; 4 tokens,
-        // 3072 rows of 4096: 5.6 with one, 6.7 with two), where their sums fit beside the planes.
+        // 3072 rows of 4096: 5.6 with one, 6.7 with two). More than 24 pairs leave no room
+        // for their sums.
         p.rt = tiles > 2048 && tokens * p.per <= 24 ? 2 : 1;
         // One round of workgroups, two on a unit where their LDS fits twice, with as many
         // turns each.
