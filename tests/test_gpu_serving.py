@@ -737,3 +737,59 @@ def test_captured_step_follows_the_lengths(gpu, kind):
         got, want = a.outputs(), b.outputs()
         for name in want:
             assert np.array_equal(got[name], want[name]), (turn, name)
+
+
+class Chunk:
+    """Products, append and attention of a chunk of tokens, with scratch of their own."""
+
+    def __init__(self, gpu, kind, count, rng):
+        self.gpu, self.count = gpu, count
+        self.cols, self.rows, self.group = 2048, 6 * 128, 32
+        self.seq = so.Sequences(gpu, kind, 128, 4, 1, 64, [700 + count], rng)
+        self.packed = so.q4_on_device(gpu, *so.q4_random(rng, self.rows, self.cols, self.group),
+                                      self.group)
+        k, v = (rng.normal(size=(700, 1, 128)).astype(np.float32) for _ in range(2))
+        self.seq.append(self.seq.batch([700], [700]), k, v)
+        self.batch = self.seq.batch([count], [700 + count])
+        self.x = lh.DeviceBuffer(4 * count * self.cols)
+        self.qkv = lh.DeviceBuffer(4 * count * self.rows)
+        self.out = lh.DeviceBuffer(4 * count * 512)
+        self.sizes = [gpu.lh_q4_scratch(self.cols, count), gpu.lh_paged_attention_scratch(
+            ctypes.byref(self.seq.cache), ctypes.byref(self.batch), 4)]
+        self.scratch = lh.DeviceBuffer(max(self.sizes + [16]))
+
+    def step(self, stream):
+        g, n, size = self.gpu, self.count, self.scratch.nbytes
+        cache, batch = ctypes.byref(self.seq.cache), ctypes.byref(self.batch)
+        q = self.qkv.ptr
+        lh.check(g.lh_q4_matvec(self.packed.ptr, self.x.ptr, self.cols, q, self.rows, self.rows,
+                                self.cols, self.group, n, self.scratch.ptr, size, stream))
+        lh.check(g.lh_paged_append(cache, batch, 4, q, self.rows, q + 2048, self.rows, q + 2560,
+                                   self.rows, None, None, 0, None, q, self.rows, stream))
+        lh.check(g.lh_paged_attention(cache, batch, 4, q, self.rows, 0.0625, self.out.ptr, 512,
+                                      self.scratch.ptr, size, stream))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("counts", [(5, 40), (100, 150)])
+def test_captured_chunks_on_two_streams(gpu, kind, counts):
+    """Two captured chunks replayed at once, again and again, equal eager ones."""
+    chunks = [Chunk(gpu, kind, c, np.random.default_rng(c)) for c in counts]
+    eager = [Chunk(gpu, kind, c, np.random.default_rng(c)) for c in counts]
+    graphs = [Graph(c.step) for c in chunks]
+    rng = np.random.default_rng(1)
+    for turn in range(4):
+        for c, e in zip(chunks, eager):
+            x = rng.normal(size=(c.count, c.cols)).astype(np.float32)
+            c.x.upload(x)
+            e.x.upload(x)
+        for g in graphs:
+            assert g.hip.hipGraphLaunch(g.exec, ctypes.c_void_p(g.stream)) == 0
+        for e in eager:
+            e.step(None)
+        lh.check(gpu.lh_device_synchronize())
+        for c, e in zip(chunks, eager):
+            want = e.out.download(np.float32)
+            assert np.isfinite(want).all()
+            assert np.array_equal(c.out.download(np.float32), want), turn
+            assert np.array_equal(c.qkv.download(np.float32), e.qkv.download(np.float32)), turn
