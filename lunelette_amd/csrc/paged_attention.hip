@@ -130,7 +130,7 @@ struct PromptRows {
     float cs[2], qs[2], m[2], sum[2], offset[2];
     int32_t limit[2], low, high;
     floatx4 acc[2][D / 16];
-    float shift;
+    float shift[2];   // of value scales: a column's own, so no row's goes by what it hides
     bool lost[2];
     uint32_t g, lane;
 
@@ -225,23 +225,6 @@ struct PromptRows {
         }
         if (Q4) {
             scales(b, 2, scale, z);
-            float most = 0;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                most = fmaxf(most, scale[e]);
-            }
-            // shift * scale stays below P_SCALE; a larger scale than so far lowers it.
-            if (__ballot(most * shift >= P_SCALE)) {
-                const float next = value_shift(column_max(most), shift), ratio = next / shift;
-#pragma unroll
-                for (int n = 0; n < 2; n++) {
-#pragma unroll
-                    for (int i = 0; i < D / 16; i++) {
-                        acc[n][i] *= ratio;
-                    }
-                }
-                shift = next;
-            }
         }
         f16x8 ph[2], pl[2];
 #pragma unroll
@@ -250,7 +233,7 @@ struct PromptRows {
             float vs[8], vz[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                vs[e] = Q4 ? scale[e] * shift : 0.0f;
+                vs[e] = Q4 ? scale[e] : 0.0f;
                 vz[e] = z[e];
             }
             if (Q4 && edge) {
@@ -258,8 +241,25 @@ struct PromptRows {
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const bool hidden = position(base, e) > limit[n];
-                    vs[e] = hidden ? 0.0f : vs[e];   // may be a NaN
+                    vs[e] = hidden ? 0.0f : vs[e];   // may hold anything
                     vz[e] = hidden ? 0.0f : vz[e];
+                }
+            }
+            if (Q4) {
+                float most = 0;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    most = fmaxf(most, vs[e]);
+                }
+                // shift * scale stays below P_SCALE; a larger scale than so far lowers it.
+                if (__ballot(most * shift[n] >= P_SCALE)) {
+                    const float next = value_shift(column_max(most), shift[n]);
+                    const float ratio = next / shift[n];
+#pragma unroll
+                    for (int i = 0; i < D / 16; i++) {
+                        acc[n][i] *= ratio;
+                    }
+                    shift[n] = next;
                 }
             }
 #pragma unroll
@@ -268,7 +268,7 @@ struct PromptRows {
                 sum[n] += p[n][e];
                 if (Q4) {
                     offset[n] = __builtin_fmaf(p[n][e], vz[e], offset[n]);
-                    p[n][e] *= vs[e];
+                    p[n][e] *= vs[e] * shift[n];
                 } else {
                     p[n][e] *= P_SCALE;
                 }
@@ -486,12 +486,12 @@ k_paged_prompt(AttentionArgs a)
             c.limit[n] = limit_of(row_of(n));
             c.m[n] = -__builtin_inff();
             c.sum[n] = c.offset[n] = 0;
+            c.shift[n] = exp2i(123);
 #pragma unroll
             for (int i = 0; i < D / 16; i++) {
                 c.acc[n][i] = (floatx4){0, 0, 0, 0};
             }
         }
-        c.shift = exp2i(123);
         // Limits do not fall from a row to the next.
         c.low = __builtin_amdgcn_readlane(c.limit[0], 0);
         c.high = __builtin_amdgcn_readlane(c.limit[1], 15);
@@ -543,10 +543,10 @@ k_paged_prompt(AttentionArgs a)
             __syncthreads();
         }
         floatx4* joined = reinterpret_cast<floatx4*>(buffers) + wave * (D / 8) * 64 + lane;
-        const float back = Q4 ? 1.0f / c.shift : 1.0f / P_SCALE;   // powers of two
         float sum[2];
 #pragma unroll
         for (int n = 0; n < 2; n++) {
+            const float back = Q4 ? 1.0f / c.shift[n] : 1.0f / P_SCALE;   // powers of two
             sum[n] = c.lost[n] ? __builtin_nanf("") : column_sum(c.sum[n]);
             const float offset = Q4 ? column_sum(c.offset[n]) : 0.0f;
 #pragma unroll

@@ -1,0 +1,46 @@
+"""The batched serving operators on the GPU where values differ by many powers of two
+or are not finite: what a token does not see, unlikely positions, the largest keys, and
+rows whose elements span the range of FP32."""
+import numpy as np
+import pytest
+
+import lunelette_amd as lh
+
+import serving_oracle as so
+from test_gpu_serving import KINDS, close
+
+pytestmark = pytest.mark.gpu
+
+# (head dim, query heads, tokens, positions before them): a tile of a prompt from its
+# start and after a prefix, and each of the tiles of few rows.
+CALLS = [(128, 3, 48, 0), (64, 4, 40, 75), (64, 2, 150, 20), (128, 1, 16, 75), (64, 1, 7, 30),
+         (128, 1, 3, 40), (64, 4, 1, 100)]
+
+
+def filled(gpu, kind, dim, heads, k, v, page=32):
+    """A sequence of one KV head with these keys and values [n][dim], and what the
+    cache holds of them."""
+    n = k.shape[0]
+    seq = so.Sequences(gpu, kind, dim, heads, 1, page, [n], np.random.default_rng(n))
+    seq.append(seq.batch([n], [n]), k[:, None], v[:, None])
+    return seq, so.cache_values(k[:, None], kind), so.cache_values(v[:, None], kind)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,heads,count,prefix", CALLS[:-1])
+@pytest.mark.parametrize("power", [13, 24, 60, 100])
+def test_paged_hidden_values_take_no_part(gpu, kind, dim, heads, count, prefix, power):
+    """A value far larger than the others at a position that only the last tokens
+    see: the tokens before it keep their precision."""
+    if kind == lh.CACHE_F16 and power > 13:
+        pytest.skip("past FP16")
+    rng = np.random.default_rng(dim + count)
+    n = prefix + count
+    k, v = (rng.normal(size=(n, dim)).astype(np.float32) for _ in range(2))
+    v[n - 2] *= np.float32(2.0 ** power)
+    seq, keys, values = filled(gpu, kind, dim, heads, k, v)
+    q = rng.normal(size=(count, heads, dim)).astype(np.float32)
+    got = seq.attention(seq.batch([count], [n]), q, 0.125)
+    for t in range(count):
+        want, off = so.attention(q[t], keys, values, prefix + t, 0.125)
+        close(got[t], want, off)
