@@ -145,9 +145,10 @@ size_t lh_paged_attention_scratch(const lh_paged_cache *cache, const lh_paged_ba
  * nothing and gives 0; one that sees a position without a place in the cache
  * gives NaN, as does one that sees a key with an Inf or NaN, or a value with one
  * (in FP16 pages in that element alone). What no token sees may hold anything.
- * Products are formed from queries (and probabilities, times the values' scales)
- * as two FP16 planes, which keep them to 2^-22 of themselves or 2^-38 of the
- * largest; sums and the softmax are FP32. */
+ * Products are formed from two FP16 planes: of queries, which keep them to 2^-22
+ * of themselves or 2^-38 of their row's largest, and of probabilities (in 4-bit pages
+ * times their values' scales), 2^-22 of themselves or 2^-32 of the row's largest of
+ * these. Sums and the softmax are FP32. */
 int lh_paged_attention(const lh_paged_cache *cache, const lh_paged_batch *batch, uint32_t heads,
     const float *d_q, size_t q_stride, float scale, float *d_out, size_t out_stride,
     void *d_scratch, size_t scratch_bytes, void *stream);

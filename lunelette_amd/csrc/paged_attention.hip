@@ -46,16 +46,33 @@ __device__ __forceinline__ float column_sum(float v)
 // The reference of a column's softmax need not be its maximum: it follows once that is
 // SLACK (in powers of two) above, so the sums are seldom rescaled (with every new
 // maximum some column of a wave had one in most blocks: 62.6 against 57.1 us for 256
-// tokens after 4096 positions).
-// Probabilities then reach 2^SLACK, their planes 2^SLACK * P_SCALE = 2^14; what a plane
-// drops is below 2^-31 of the reference.
-constexpr float SLACK = 8, P_SCALE = 64;
+// tokens after 4096 positions). Probabilities are formed relative to 2^SLACK times the
+// reference and stay up to 1 (and a rounding).
+//
+// The second product takes them (in 4-bit pages times their positions' value scales) times
+// a power of two that keeps its planes below 2^15: P_SCALE, or in 4-bit pages one that
+// each column lowers when a product of a probability and a scale comes to P_LIMIT. Such a
+// product then stands in [2^7, 2^8), and later ones have 2^8 to grow as probabilities
+// do. A plane ends at 2^-25: 2^-32 of the largest probability, or product.
+constexpr float SLACK = 8, P_SCALE = 32768, P_LIMIT = 32768;
 
-// The power of two that takes value scales up to `most` below P_SCALE, at most `now`.
+// The power of two that takes a product `most` to [2^7, 2^8), at most `now`.
 __device__ __forceinline__ float value_shift(float most, float now)
 {
     const int e = (int)((__float_as_uint(most) >> 23) & 0xffu) - 127;
-    return fminf(now, exp2i(e < -118 ? 123 : 5 - e));
+    return fminf(now, exp2i(e < -116 ? 123 : 7 - e));
+}
+
+// A column's reference falls by 2^down (<= 0, -Inf for its first): the products so far are
+// that much less, so their power of two may rise as much, to 2^123. The factor of their
+// sums in the new units.
+__device__ __forceinline__ float raise_shift(float& shift, float down)
+{
+    const uint32_t bits = __float_as_uint(shift);
+    const float room = (float)(123 + 127 - (int)(bits >> 23));
+    const float up = fminf(-__builtin_floorf(down), room);
+    shift = __uint_as_float(bits + ((uint32_t)(int)up << 23));
+    return __builtin_amdgcn_exp2f(down + up);
 }
 
 struct AttentionArgs {
@@ -130,7 +147,7 @@ struct PromptRows {
     float cs[2], qs[2], m[2], sum[2], offset[2];
     int32_t limit[2], low, high;
     floatx4 acc[2][D / 16];
-    float shift[2];   // of value scales: a column's own, so no row's goes by what it hides
+    float shift[2];   // of the products of probabilities and value scales, a column's own
     bool lost[2];
     uint32_t g, lane;
 
@@ -212,14 +229,15 @@ struct PromptRows {
             }
             most = fmaxf(column_max(most) * cs[n], m[n]);
             if (__ballot(most > m[n] + SLACK)) {
-                const float keep = m[n] > -__builtin_inff() ? __builtin_amdgcn_exp2f(m[n] - most)
-                    : 0.0f;
+                const float down = m[n] > -__builtin_inff() ? m[n] - most : -__builtin_inff();
+                const float keep = __builtin_amdgcn_exp2f(down);
+                const float products = Q4 ? raise_shift(shift[n], down) : keep;
                 m[n] = most;
                 sum[n] *= keep;
                 offset[n] *= keep;
 #pragma unroll
                 for (int i = 0; i < D / 16; i++) {
-                    acc[n][i] *= keep;
+                    acc[n][i] *= products;
                 }
             }
         }
@@ -229,7 +247,7 @@ struct PromptRows {
         f16x8 ph[2], pl[2];
 #pragma unroll
         for (int n = 0; n < 2; n++) {
-            const float top = m[n] > -__builtin_inff() ? m[n] : 0.0f;
+            const float top = (m[n] > -__builtin_inff() ? m[n] : 0.0f) + SLACK;
             float vs[8], vz[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
@@ -245,14 +263,24 @@ struct PromptRows {
                     vz[e] = hidden ? 0.0f : vz[e];
                 }
             }
-            if (Q4) {
-                float most = 0;
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    most = fmaxf(most, vs[e]);
+            for (int e = 0; e < 8; e++) {
+                p[n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[n][e], cs[n], -top));
+                sum[n] += p[n][e];
+                if (Q4) {
+                    offset[n] = __builtin_fmaf(p[n][e], vz[e], offset[n]);
+                    p[n][e] *= vs[e];
+                } else {
+                    p[n][e] *= P_SCALE;
                 }
-                // shift * scale stays below P_SCALE; a larger scale than so far lowers it.
-                if (__ballot(most * shift[n] >= P_SCALE)) {
+            }
+            if (Q4) {
+                float most = p[n][0];
+#pragma unroll
+                for (int e = 1; e < 8; e++) {
+                    most = fmaxf(most, p[n][e]);
+                }
+                if (__ballot(most * shift[n] >= P_LIMIT)) {
                     const float next = value_shift(column_max(most), shift[n]);
                     const float ratio = next / shift[n];
 #pragma unroll
@@ -261,16 +289,9 @@ struct PromptRows {
                     }
                     shift[n] = next;
                 }
-            }
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                p[n][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[n][e], cs[n], -top));
-                sum[n] += p[n][e];
-                if (Q4) {
-                    offset[n] = __builtin_fmaf(p[n][e], vz[e], offset[n]);
-                    p[n][e] *= vs[e] * shift[n];
-                } else {
-                    p[n][e] *= P_SCALE;
+                for (int e = 0; e < 8; e++) {
+                    p[n][e] *= shift[n];
                 }
             }
             planes8(p[n], ph[n], pl[n]);
@@ -773,7 +794,6 @@ struct Decode {
     {
         float scale[C], z[C];
         if (Q4) {
-            float most = 0;
 #pragma unroll
             for (int e = 0; e < C; e++) {
                 const uint32_t word = step.vs[e >> 2][e & 3];
@@ -782,17 +802,6 @@ struct Decode {
                 if (edge && position(base, e) > limit) {
                     scale[e] = z[e] = 0;   // may hold anything
                 }
-                most = fmaxf(most, scale[e]);
-            }
-            // shift * scale stays below P_SCALE; a larger scale than so far lowers it.
-            if (__ballot(most * shift >= P_SCALE)) {
-                most = column_max(most);
-                const float next = value_shift(most, shift), ratio = next / shift;
-#pragma unroll
-                for (int i = 0; i < D / 16; i++) {
-                    acc[i] *= ratio;
-                }
-                shift = next;
             }
         }
         if (edge) {
@@ -808,25 +817,46 @@ struct Decode {
         }
         most = fmaxf(column_max(most) * cs, m);
         if (__ballot(most > m + SLACK)) {
-            const float keep = m > -__builtin_inff() ? __builtin_amdgcn_exp2f(m - most) : 0.0f;
+            const float down = m > -__builtin_inff() ? m - most : -__builtin_inff();
+            const float keep = __builtin_amdgcn_exp2f(down);
+            const float products = Q4 ? raise_shift(shift, down) : keep;
             m = most;
             sum *= keep;
             offset *= keep;
 #pragma unroll
             for (int i = 0; i < D / 16; i++) {
-                acc[i] *= keep;
+                acc[i] *= products;
             }
         }
-        const float top = m > -__builtin_inff() ? m : 0.0f;
+        const float top = (m > -__builtin_inff() ? m : 0.0f) + SLACK;
 #pragma unroll
         for (int e = 0; e < C; e++) {
             p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[e], cs, -top));
             sum += p[e];
             if (Q4) {
                 offset = __builtin_fmaf(p[e], z[e], offset);
-                p[e] *= scale[e] * shift;
+                p[e] *= scale[e];
             } else {
                 p[e] *= P_SCALE;
+            }
+        }
+        if (Q4) {
+            most = p[0];
+#pragma unroll
+            for (int e = 1; e < C; e++) {
+                most = fmaxf(most, p[e]);
+            }
+            if (__ballot(most * shift >= P_LIMIT)) {
+                const float next = value_shift(column_max(most), shift), ratio = next / shift;
+#pragma unroll
+                for (int i = 0; i < D / 16; i++) {
+                    acc[i] *= ratio;
+                }
+                shift = next;
+            }
+#pragma unroll
+            for (int e = 0; e < C; e++) {
+                p[e] *= shift;
             }
         }
 #pragma unroll

@@ -44,3 +44,39 @@ def test_paged_hidden_values_take_no_part(gpu, kind, dim, heads, count, prefix, 
     for t in range(count):
         want, off = so.attention(q[t], keys, values, prefix + t, 0.125)
         close(got[t], want, off)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,heads,count,prefix", CALLS)
+@pytest.mark.parametrize("where", ["first", "middle", "raised"])
+def test_paged_unlikely_positions_take_no_part(gpu, kind, dim, heads, count, prefix, where):
+    """A visible position of hardly any probability (e^-40) whose value is far larger
+    than the others costs them no precision, whether it comes before them, among them,
+    or had nearly all of the probability until they came."""
+    rng = np.random.default_rng(dim + count + len(where))
+    before = 70
+    n = before + prefix + count
+    k = np.zeros((n, dim), np.float32)
+    v = rng.normal(size=(n, dim)).astype(np.float32)
+    at = {"first": 3, "middle": 45, "raised": 10}[where]
+    # Scores 0 and -40; "raised": 0 up to position 39 and 40 from there on.
+    if where == "raised":
+        k[40:, 0] = 320
+    else:
+        k[at, 0] = -320
+    v[at] *= np.float32(2.0 ** (13 if kind == lh.CACHE_F16 else 30))
+    seq, keys, values = filled(gpu, kind, dim, heads, k, v)
+    q = np.zeros((count, heads, dim), np.float32)
+    q[..., 0] = 1
+    got = seq.attention(seq.batch([count], [n]), q, 0.125)
+    for t in range(count):
+        last = before + prefix + t
+        want, _ = so.attention(q[t], keys, values, last, 0.125)
+        # Equal scores of all positions that count: the exponential's two steps, the
+        # sums, and planes to 2^-31 of the largest product at each position.
+        p = np.exp((keys[:last + 1, 0, 0].astype(np.float64) -
+                    keys[:last + 1, 0, 0].max()) * 0.125)
+        p /= p.sum()
+        size = p @ (3 * np.abs(values[:last + 1, 0]).max(-1).astype(np.float64))
+        off = size * (2.0 ** -20 + ((last + 1) / 16 + 64) * so.EPS32)
+        close(got[t], want, np.full_like(want, off))
