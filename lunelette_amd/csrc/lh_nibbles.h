@@ -69,4 +69,28 @@ __device__ __forceinline__ void planes8(const float* v, f16x8& hi, f16x8& lo)
     lo = __builtin_bit_cast(f16x8, l);
 }
 
+// Eight values as planes of which the first lies away from 0 by up to a step and the
+// second, of the other sign, has the rest: 22 bits where planes8 has 23. Times an
+// infinite number the two are Inf and -Inf, so their sum is a NaN whatever the value's
+// sign and bits are (planes8 gives an Inf where both have the same sign).
+__device__ __forceinline__ void planes8_away(const float* v, f16x8& hi, f16x8& lo)
+{
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    u32x4 h, l;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float a = v[2 * i], b = v[2 * i + 1];
+        // Toward 0, then the next magnitude.
+        h[i] = __builtin_bit_cast(uint32_t,
+            __builtin_bit_cast(u16x2, __builtin_amdgcn_cvt_pkrtz(a, b)) + (u16x2){1, 1});
+        float ra, rb;
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(ra) : "v"(h[i]), "v"(a));
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+            : "=v"(rb) : "v"(h[i]), "v"(b));
+        l[i] = __builtin_bit_cast(uint32_t, (f16x2){(_Float16)ra, (_Float16)rb});
+    }
+    hi = __builtin_bit_cast(f16x8, h);
+    lo = __builtin_bit_cast(f16x8, l);
+}
+
 }  // namespace lh

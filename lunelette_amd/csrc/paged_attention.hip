@@ -99,7 +99,9 @@ __device__ __forceinline__ int32_t split_chunk(const AttentionArgs& a, int32_t s
 // A lane's part of a query row: dims 32 j + 8 g .. + 7, scaled by a power of two so
 // that the row's largest lies in [2^14, 2^15), in planes; cs takes a score in units
 // of that back (times log2 e), qs is the row's sum in them.
-template <int D>
+// FP16 keys may have an Inf, which has to make the score a NaN: a score of -Inf would be
+// left out of the softmax as a hidden position is.
+template <int D, bool Q4>
 __device__ __forceinline__ void load_query(const float* q, uint32_t g, float scale,
     f16x8 (&hi)[D / 32], f16x8 (&lo)[D / 32], float& cs, float& qs)
 {
@@ -125,7 +127,11 @@ __device__ __forceinline__ void load_query(const float* q, uint32_t g, float sca
     }
 #pragma unroll
     for (int j = 0; j < D / 32; j++) {
-        planes8(v + 8 * j, hi[j], lo[j]);
+        if (Q4) {
+            planes8(v + 8 * j, hi[j], lo[j]);
+        } else {
+            planes8_away(v + 8 * j, hi[j], lo[j]);
+        }
     }
     qs = column_sum(sum);
     // Never 0 or Inf, which an infinite or a zero score would turn into NaN.
@@ -527,7 +533,7 @@ k_paged_prompt(AttentionArgs a)
 #pragma unroll
         for (int n = 0; n < 2; n++) {
             const int64_t row = row_of(n);
-            load_query<D>(a.q + (size_t)(span.begin + row / a.group) * a.q_stride +
+            load_query<D, Q4>(a.q + (size_t)(span.begin + row / a.group) * a.q_stride +
                 ((size_t)h * a.group + row % a.group) * D, c.g, a.scale, c.hi[n], c.lo[n], c.cs[n],
                 c.qs[n]);
         }
@@ -1021,7 +1027,7 @@ k_paged_decode(AttentionArgs a)
             ((size_t)h * a.group + row % a.group) * D;
         if constexpr (Decode<D, Q4, C>::SHARED) {
             f16x8 hi[D / 32], lo[D / 32];
-            load_query<D>(q, c.g, a.scale, hi, lo, c.cs, c.qs);
+            load_query<D, Q4>(q, c.g, a.scale, hi, lo, c.cs, c.qs);
             __syncthreads();   // the previous tile's readers
             if (wave == 0) {
 #pragma unroll
@@ -1032,7 +1038,7 @@ k_paged_decode(AttentionArgs a)
             }
             __syncthreads();
         } else {
-            load_query<D>(q, c.g, a.scale, c.hi, c.lo, c.cs, c.qs);
+            load_query<D, Q4>(q, c.g, a.scale, c.hi, c.lo, c.cs, c.qs);
         }
         int32_t turn = 0;
         if constexpr (Q4) {

@@ -80,3 +80,45 @@ def test_paged_unlikely_positions_take_no_part(gpu, kind, dim, heads, count, pre
         size = p @ (3 * np.abs(values[:last + 1, 0]).max(-1).astype(np.float64))
         off = size * (2.0 ** -20 + ((last + 1) / 16 + 64) * so.EPS32)
         close(got[t], want, np.full_like(want, off))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,heads,count,prefix", CALLS)
+@pytest.mark.parametrize("at", [0, 10, 45])
+@pytest.mark.parametrize("inf", [np.inf, -np.inf, 7e4])
+def test_paged_infinite_keys(gpu, kind, dim, heads, count, prefix, at, inf):
+    """Tokens that see a key with an Inf (or what FP16 rounds to it) give NaN,
+    whatever the sign and size of their queries there; the others do not notice."""
+    rng = np.random.default_rng(dim + count + at)
+    before = 70 if prefix or count == 1 else 0
+    n = before + prefix + count
+    k, v = (rng.normal(size=(n, dim)).astype(np.float32) for _ in range(2))
+    k[at, 5] = inf
+    seq, keys, values = filled(gpu, kind, dim, heads, k, v)
+    q = rng.normal(size=(count, heads, dim)).astype(np.float32)
+    q[..., 5] = np.ldexp(q[..., 5], -rng.integers(0, 45, size=(count, heads)))
+    q[-1, 0, 5] = 0
+    got = seq.attention(seq.batch([count], [n]), q, 0.125)
+    if np.isfinite(keys).all():
+        return   # 4 bits hold 7e4
+    for t in range(count):
+        last = before + prefix + t
+        if last >= at:
+            assert np.isnan(got[t]).all(), t
+            continue
+        want, off = so.attention(q[t], keys, values, last, 0.125)
+        close(got[t], want, off)
+
+
+@pytest.mark.parametrize("dim,heads,count,prefix", CALLS)
+def test_paged_largest_halves(gpu, dim, heads, count, prefix):
+    """FP16's largest keys and values are finite."""
+    rng = np.random.default_rng(dim + count)
+    n = 70 + prefix + count
+    k, v = (rng.choice(np.float32([-65504, 65504, 1]), size=(n, dim)) for _ in range(2))
+    seq, keys, values = filled(gpu, lh.CACHE_F16, dim, heads, k, v)
+    q = (rng.normal(size=(count, heads, dim)) * 1e-5).astype(np.float32)
+    got = seq.attention(seq.batch([count], [n]), q, 0.125)
+    for t in range(count):
+        want, off = so.attention(q[t], keys, values, 70 + prefix + t, 0.125)
+        close(got[t], want, off)
