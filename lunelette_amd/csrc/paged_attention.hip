@@ -75,6 +75,14 @@ __device__ __forceinline__ float raise_shift(float& shift, float down)
     return __builtin_amdgcn_exp2f(down + up);
 }
 
+// An infinite FP16 value leaves Inf or NaN in its element's sum, by its sign and those of
+// the probabilities' planes: NaN it is. (Finite ones cannot overflow: 2^15 * 2^16 each.)
+template <bool Q4>
+__device__ __forceinline__ float nan_if_odd(float v)
+{
+    return Q4 ? v : __builtin_fmaf(v, 0.0f, v);
+}
+
 struct AttentionArgs {
     Pages cache;
     Batch batch;
@@ -580,7 +588,8 @@ k_paged_prompt(AttentionArgs a)
             for (int i = 0; i < D / 16; i++) {
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    c.acc[n][i][r] = __builtin_fmaf(c.acc[n][i][r], back, offset);
+                    c.acc[n][i][r] = nan_if_odd<Q4>(
+                        __builtin_fmaf(c.acc[n][i][r], back, offset));
                 }
                 if (team) {
                     joined[(n * (D / 16) + i) * 64] = c.acc[n][i];
@@ -1104,7 +1113,8 @@ k_paged_decode(AttentionArgs a)
             floatx4 y;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                y[r] = __builtin_fmaf(c.acc[i][r], back, Q4 ? c.offset * keep : 0.0f);
+                y[r] = nan_if_odd<Q4>(
+                    __builtin_fmaf(c.acc[i][r], back, Q4 ? c.offset * keep : 0.0f));
             }
             *reinterpret_cast<floatx4*>(&joined[wave][lane & 15][16 * i + 4 * c.g]) = y;
         }

@@ -122,3 +122,27 @@ def test_paged_largest_halves(gpu, dim, heads, count, prefix):
     for t in range(count):
         want, off = so.attention(q[t], keys, values, 70 + prefix + t, 0.125)
         close(got[t], want, off)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,heads,count,prefix", CALLS)
+@pytest.mark.parametrize("at", [0, 10, 45])
+@pytest.mark.parametrize("inf", [np.inf, -np.inf])
+def test_paged_infinite_values(gpu, kind, dim, heads, count, prefix, at, inf):
+    """Tokens that see a value with an Inf give NaN, of FP16 pages in that element
+    alone."""
+    rng = np.random.default_rng(dim + count + at)
+    before = 70 if prefix or count == 1 else 0
+    n = before + prefix + count
+    k, v = (rng.normal(size=(n, dim)).astype(np.float32) for _ in range(2))
+    v[at, 5] = inf
+    seq, keys, values = filled(gpu, kind, dim, heads, k, v)
+    q = rng.normal(size=(count, heads, dim)).astype(np.float32)
+    got = seq.attention(seq.batch([count], [n]), q, 0.125)
+    finite = np.where(np.isfinite(values), values, 0)
+    for t in range(count):
+        last = before + prefix + t
+        want, off = so.attention(q[t], keys, finite, last, 0.125)
+        if last >= at:
+            want[:, 5 if kind == lh.CACHE_F16 else slice(None)] = np.nan
+        close(got[t], want, off)
