@@ -148,7 +148,8 @@ size_t lh_paged_attention_scratch(const lh_paged_cache *cache, const lh_paged_ba
  * Products are formed from two FP16 planes: of queries, which keep them to 2^-22
  * of themselves or 2^-38 of their row's largest, and of probabilities (in 4-bit pages
  * times their values' scales), 2^-22 of themselves or 2^-32 of the row's largest of
- * these. Sums and the softmax are FP32. */
+ * these. Sums and the softmax are FP32: scores, and a row's number of positions
+ * times its largest value, have to lie in its range. */
 int lh_paged_attention(const lh_paged_cache *cache, const lh_paged_batch *batch, uint32_t heads,
     const float *d_q, size_t q_stride, float scale, float *d_out, size_t out_stride,
     void *d_scratch, size_t scratch_bytes, void *stream);

@@ -142,8 +142,10 @@ __device__ __forceinline__ void load_query(const float* q, uint32_t g, float sca
         }
     }
     qs = column_sum(sum);
-    // Never 0 or Inf, which an infinite or a zero score would turn into NaN.
-    cs = fminf(fmaxf(scale * exp2i(-e2), 1e-37f), 3e38f);
+    // Never 0 or Inf, which a hidden or a zero score would turn into NaN. Scores of FP16 keys
+    // are below 2^39, so they vanish before cs does; 4-bit keys reach 2^128 and meet cs (to
+    // 2^-150), or KEY_UNIT, before the sums, so that any score that FP32 holds is formed.
+    cs = fminf(fmaxf(scale * exp2i(-e2), 0x1p-149f), 3e38f);
 }
 
 // Prompts: four waves with 32 query rows each (two column tiles) share every block of 32
@@ -373,6 +375,12 @@ struct PromptRows {
     }
 };
 
+// Of the scales and zeros of a prompt's 4-bit keys in LDS: with keys up to 2^128 their
+// products with a query's sums (up to 2^25) stay in FP32's range, and keys count to 2^-125.
+// (Meeting cs before the sums, as in the decode kernel, takes 32 instructions a block here:
+// 55.9 against 55.1 us for 256 tokens after 4096.)
+constexpr float KEY_UNIT = 0x1p-24f;
+
 enum { PROMPT_ROWS = 128 };
 
 // grid (KV heads, sequences, tiles of the splits in turn): the tiles of a KV head of
@@ -481,8 +489,10 @@ k_paged_prompt(AttentionArgs a)
                 }
             }
             if (wave == 0) {
-                float scale = bf16_to_f32(words & 0xffffu);
-                float z = __builtin_fmaf(8.0f, scale, __uint_as_float(words & 0xffff0000u));
+                const float unit = lane < 32 ? KEY_UNIT : 1.0f;
+                float scale = bf16_to_f32(words & 0xffffu) * unit;
+                float z = __builtin_fmaf(8.0f, scale,
+                    __uint_as_float(words & 0xffff0000u) * unit);
                 if (32 * b + (int32_t)(lane & 31) > high) {
                     scale = z = 0;   // may hold anything
                 }
@@ -544,6 +554,9 @@ k_paged_prompt(AttentionArgs a)
             load_query<D, Q4>(a.q + (size_t)(span.begin + row / a.group) * a.q_stride +
                 ((size_t)h * a.group + row % a.group) * D, c.g, a.scale, c.hi[n], c.lo[n], c.cs[n],
                 c.qs[n]);
+            if (Q4) {
+                c.cs[n] = fminf(c.cs[n] / KEY_UNIT, 3e38f);
+            }
         }
         if (Q4 && first < end) {
             decode(first, blocks[0]);
@@ -744,7 +757,7 @@ struct Decode {
         return base + 16 * (PACK * (e >> 2) + (int32_t)u) + 4 * (int32_t)g + (e & 3);
     }
 
-    // Scores of the lane's positions, in units of 1 / cs.
+    // Scores of the lane's positions, of FP16 keys in units of 1 / cs.
     __device__ __forceinline__ void scores(const Step& step, float (&p)[C])
     {
         floatx4 s[4];
@@ -795,7 +808,7 @@ struct Decode {
                     const float scale = bf16_to_f32(word & 0xffffu);
                     const float z = __builtin_fmaf(8.0f, scale,
                         __uint_as_float(word & 0xffff0000u));
-                    y = __builtin_fmaf(z, qs, scale * y);
+                    y = __builtin_fmaf(z * cs, qs, scale * cs * y);
                 }
                 p[4 * w + i] = y;
             }
@@ -830,7 +843,7 @@ struct Decode {
         for (int e = 1; e < C; e++) {
             most = fmaxf(most, p[e]);
         }
-        most = fmaxf(column_max(most) * cs, m);
+        most = fmaxf(Q4 ? column_max(most) : column_max(most) * cs, m);
         if (__ballot(most > m + SLACK)) {
             const float down = m > -__builtin_inff() ? m - most : -__builtin_inff();
             const float keep = __builtin_amdgcn_exp2f(down);
@@ -846,7 +859,7 @@ struct Decode {
         const float top = (m > -__builtin_inff() ? m : 0.0f) + SLACK;
 #pragma unroll
         for (int e = 0; e < C; e++) {
-            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[e], cs, -top));
+            p[e] = __builtin_amdgcn_exp2f(Q4 ? p[e] - top : __builtin_fmaf(p[e], cs, -top));
             sum += p[e];
             if (Q4) {
                 offset = __builtin_fmaf(p[e], z[e], offset);

@@ -146,3 +146,38 @@ def test_paged_infinite_values(gpu, kind, dim, heads, count, prefix, at, inf):
         if last >= at:
             want[:, 5 if kind == lh.CACHE_F16 else slice(None)] = np.nan
         close(got[t], want, off)
+
+
+@pytest.mark.parametrize("dim,heads,count,prefix", CALLS)
+@pytest.mark.parametrize("power", [-110, -60, 60, 104, 110, 120])
+def test_paged_keys_of_every_size(gpu, dim, heads, count, prefix, power):
+    """4-bit keys up to the end of FP32 with queries that bring the scores back to
+    a common size."""
+    rng = np.random.default_rng(dim + count)
+    n = 70 + prefix + count
+    k, v = (rng.normal(size=(n, dim)).astype(np.float32) for _ in range(2))
+    k = np.ldexp(k, power)
+    seq, keys, values = filled(gpu, lh.CACHE_Q4, dim, heads, k, v)
+    q = np.ldexp(rng.normal(size=(count, heads, dim)).astype(np.float32), -power)
+    got = seq.attention(seq.batch([count], [n]), q, 0.125)
+    for t in range(count):
+        want, off = so.attention(q[t], keys, values, 70 + prefix + t, 0.125)
+        close(got[t], want, off)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,heads,count,prefix", CALLS)
+@pytest.mark.parametrize("size,scale", [(1e-38, 1e-20), (1e-38, 1e38), (1e38, 1e-38),
+                                        (1e-44, 1.0)])
+def test_paged_ends_of_the_scale(gpu, kind, dim, heads, count, prefix, size, scale):
+    """Queries and scales at the ends of FP32 whose scores vanish or are common ones."""
+    rng = np.random.default_rng(dim + count)
+    n = 70 + prefix + count
+    k, v = (rng.normal(size=(n, dim)).astype(np.float32) for _ in range(2))
+    seq, keys, values = filled(gpu, kind, dim, heads, k, v)
+    q = (rng.uniform(-1, 1, size=(count, heads, dim)) * size).astype(np.float32)
+    scale = float(np.float32(scale))
+    got = seq.attention(seq.batch([count], [n]), q, scale)
+    for t in range(count):
+        want, off = so.attention(q[t], keys, values, 70 + prefix + t, scale)
+        close(got[t], want, off)
