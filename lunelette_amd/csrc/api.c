@@ -211,7 +211,7 @@ void lh_event_destroy(void *event)
 static int launched(int status, const char *what)
 {
     if (status) {
-        lh_set_error("%s launch failed: %s", what, hipGetErrorString(hipGetLastError()));
+        lh_set_error("%s launch failed: %s", what, lh_launch_text(status));
         return -1;
     }
     return 0;

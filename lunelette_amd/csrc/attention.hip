@@ -135,7 +135,7 @@ extern "C" int lh_launch_step_embed(const uint16_t* E, const float* yarn, int32_
     static_assert(LH_HIDDEN == 3 * 256 * 4, "three workgroups of four values per thread");
     hipLaunchKernelGGL(k_step_embed, dim3(3), dim3(256), 0, s, E, yarn, id, length, qfactor,
         params, x);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }
 
 #ifndef LH_ATTN_FUSED_BLOCKS
@@ -183,11 +183,18 @@ extern "C" int lh_attention_xcd_probe(uint32_t* d_words, size_t words, int* ok, 
         hipLaunchKernelGGL(lh::k_xcd_probe, dim3(g), dim3(64), 0, s, d_words + at);
         at += g;
     }
-    if (hipGetLastError() != hipSuccess ||
-        hipMemcpyAsync(host, d_words, at * sizeof(uint32_t), hipMemcpyDeviceToHost, s) != hipSuccess ||
-        hipMemsetAsync(d_words, 0, words * sizeof(uint32_t), s) != hipSuccess ||
-        hipStreamSynchronize(s) != hipSuccess) {
-        return -1;
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess) {
+        e = hipMemcpyAsync(host, d_words, at * sizeof(uint32_t), hipMemcpyDeviceToHost, s);
+    }
+    if (e == hipSuccess) {
+        e = hipMemsetAsync(d_words, 0, words * sizeof(uint32_t), s);
+    }
+    if (e == hipSuccess) {
+        e = hipStreamSynchronize(s);
+    }
+    if (e != hipSuccess) {
+        return (int)e;
     }
     int good = 1;
     at = 0;
@@ -265,7 +272,7 @@ extern "C" int lh_launch_attention(const float* q, const float* kcache_layer,
         hipLaunchKernelGGL(k_attn_combine, dim3(LH_HEADS * 4, count), dim3(256), 0, s, PM, PT, PA,
             params, capacity, out);
     }
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }
 
 // ---------------------------------------------------------------------------
@@ -333,10 +340,13 @@ extern "C" int lh_attention_noalloc(const float* d_q, const float* d_keys, const
     hipStream_t s = static_cast<hipStream_t>(stream);
     hipLaunchKernelGGL(lh::k_set_step, dim3(1), dim3(64), 0, s, params, (uint32_t)length,
         (uint32_t)count);
-    if (hipGetLastError() != hipSuccess ||
-        lh_launch_attention(d_q, d_keys, d_values, params, (uint32_t)length, (uint32_t)count,
-            (uint32_t)capacity, PM, PT, PA, nullptr, nullptr, 0ull, 0, d_out, s)) {
-        lh_set_error("attention_noalloc: launch failed");
+    int status = (int)hipGetLastError();
+    if (!status) {
+        status = lh_launch_attention(d_q, d_keys, d_values, params, (uint32_t)length,
+            (uint32_t)count, (uint32_t)capacity, PM, PT, PA, nullptr, nullptr, 0ull, 0, d_out, s);
+    }
+    if (status) {
+        lh_set_error("attention_noalloc: launch failed: %s", lh_launch_text(status));
         return -1;
     }
     return 0;
@@ -351,7 +361,7 @@ extern "C" int lh_launch_embed(const uint16_t* E, const lh_step_params* params, 
     float* x, hipStream_t s)
 {
     hipLaunchKernelGGL(k_embed, dim3(count), dim3(256), 0, s, E, params, x);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }
 
 // ---------------------------------------------------------------------------
@@ -1379,5 +1389,5 @@ extern "C" int lh_launch_attention_mfma(const float* q, const float* kcache_laye
                 splits, count, out, xs, xs_tokens, xs_scale);
         }
     }
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }

@@ -76,8 +76,10 @@ lh_workspace *lh_workspace_create(size_t capacity, size_t block)
         return NULL;
     }
     int fused = 0;
-    if (lh_attention_xcd_probe((uint32_t *)ws->d_arrive, 2 * ARRIVE_WORDS(B), &fused, NULL)) {
-        lh_set_error("workspace: XCD dispatch probe failed: %s", hipGetErrorString(hipGetLastError()));
+    const int probe = lh_attention_xcd_probe((uint32_t *)ws->d_arrive, 2 * ARRIVE_WORDS(B), &fused,
+        NULL);
+    if (probe) {
+        lh_set_error("workspace: XCD dispatch probe failed: %s", lh_launch_text(probe));
         lh_workspace_destroy(ws);
         return NULL;
     }
@@ -219,9 +221,10 @@ int lh_workspace_set_decode(lh_workspace *ws, const uint16_t *d_embedding, int64
     }
     ws->length = length;
     ws->count = 1;
-    if (lh_launch_step_embed(d_embedding, ws->d_yarn, (int32_t)id, (uint32_t)length,
-            lh_query_factor((uint32_t)length), ws->d_params, d_x, s)) {
-        lh_set_error("step embed launch failed: %s", hipGetErrorString(hipGetLastError()));
+    const int status = lh_launch_step_embed(d_embedding, ws->d_yarn, (int32_t)id,
+        (uint32_t)length, lh_query_factor((uint32_t)length), ws->d_params, d_x, s);
+    if (status) {
+        lh_set_error("step embed launch failed: %s", lh_launch_text(status));
         return -1;
     }
     return 0;
@@ -230,8 +233,7 @@ int lh_workspace_set_decode(lh_workspace *ws, const uint16_t *d_embedding, int64
 static int launched(int status, const char *what)
 {
     if (status) {
-        hipError_t e = hipGetLastError();
-        lh_set_error("%s launch failed: %s", what, hipGetErrorString(e));
+        lh_set_error("%s launch failed: %s", what, lh_launch_text(status));
         return -1;
     }
     return 0;

@@ -1,5 +1,7 @@
 /* Internal launchers between the C runtime and the gfx950 kernels. Device
- * pointers only; every launcher returns 0 or -1 (launch error). */
+ * pointers only; every launcher returns 0, the HIP error of a launch that the
+ * runtime refused (positive, taken off its record), or -1 for sizes that it does
+ * not take. */
 #ifndef LH_INTERNAL_H
 #define LH_INTERNAL_H
 
@@ -12,6 +14,12 @@
 #ifdef __cplusplus
 extern "C" {
 #endif
+
+/* A launcher's status in words. */
+static inline const char *lh_launch_text(int status)
+{
+    return status > 0 ? hipGetErrorString((hipError_t)status) : "sizes that no kernel takes";
+}
 
 /* kind: 0 FP8 codes (scaled), 1 BF16, 2 FP32. residual may be NULL. */
 int lh_launch_matvec(int kind, int lookup, const void *W, float scale, const float *x, float *y,

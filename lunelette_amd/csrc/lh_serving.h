@@ -1,5 +1,5 @@
 /* Launchers of the batched serving operators (include/lunelette_serving.h):
- * called with checked arguments, 0 or -1 (launch error). */
+ * called with checked arguments, 0 or the HIP error of a refused launch. */
 #ifndef LH_SERVING_H
 #define LH_SERVING_H
 

@@ -490,11 +490,11 @@ extern "C" int lh_launch_logprobs(const float* logits, size_t stride, uint32_t r
     const LogprobArgs a = {logits, tokens, logprob, entropy, top_logprobs, top_ids, ranges,
         reinterpret_cast<uint64_t*>(ranges + (size_t)rows * parts), stride, vocab, top, parts};
     hipLaunchKernelGGL(k_logprob_ranges, dim3(parts, rows), dim3(64 * WAVES), 0, s, a);
-    if (hipGetLastError() != hipSuccess) {
-        return -1;
+    if (const hipError_t e = hipGetLastError()) {
+        return (int)e;
     }
     if (parts > 1) {
         hipLaunchKernelGGL(k_logprob_join, dim3(rows), dim3(64 * WAVES), 0, s, a);
     }
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }

@@ -843,7 +843,7 @@ static int launch_rows(const void* W, float scale, const float* x, float* y, con
         hipLaunchKernelGGL((k_rows<KIND, LUT, NCH, R, false>), grid, dim3(256), 0, s, W, scale, x,
             y, residual, rows);
     }
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }
 
 
@@ -888,7 +888,7 @@ static int launch_generic(const void* W, float scale, const float* x, float* y,
     dim3 grid((rows + 3) / 4, tokens);
     hipLaunchKernelGGL((k_rows_generic<KIND, LUT, VEC>), grid, dim3(256), 0, s, W, scale, x, y,
         residual, rows, cols);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }
 
 template <int KIND, bool LUT>
@@ -944,7 +944,7 @@ extern "C" int lh_launch_qkv_rope(int strategy, const void* Wqkv, float sq, floa
         LH_QKV(K_FP8, false);
     }
 #undef LH_QKV
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }
 
 #ifndef LH_ATTN_FUSED_BLOCKS
@@ -995,7 +995,7 @@ extern "C" int lh_launch_qkv_attention(int lookup, const uint8_t* Wqkv, float sq
         }
     }
 #undef LH_QKV_ATTN
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }
 
 extern "C" int lh_launch_gateup_silu(int strategy, const void* Wgate, const void* Wup,
@@ -1015,7 +1015,7 @@ extern "C" int lh_launch_gateup_silu(int strategy, const void* Wgate, const void
         LH_GATEUP(K_FP8, false);
     }
 #undef LH_GATEUP
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }
 
 extern "C" int lh_launch_head(const uint16_t* E, const float* gamma, const float* xrow,
@@ -1023,7 +1023,7 @@ extern "C" int lh_launch_head(const uint16_t* E, const float* gamma, const float
 {
     hipLaunchKernelGGL(k_head, dim3(LH_VOCAB / 32), dim3(512), 0, s, E, gamma, xrow, logits,
         nonfinite);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }
 
 extern "C" int lh_launch_rmsnorm(const float* gamma, const float* x, float* out, uint32_t width,
@@ -1033,5 +1033,5 @@ extern "C" int lh_launch_rmsnorm(const float* gamma, const float* x, float* out,
         return -1;
     }
     hipLaunchKernelGGL(k_rmsnorm, dim3(tokens), dim3(64), 0, s, gamma, x, out, width);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }

@@ -765,14 +765,18 @@ k_combine_residual(const float* __restrict__ partial, size_t split_stride, size_
 
 using namespace lh;
 
-static int launched_ok(const char* what)
+static int launched(int status, const char* what)
 {
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) {
-        lh_set_error("%s launch failed: %s", what, hipGetErrorString(e));
+    if (status) {
+        lh_set_error("%s launch failed: %s", what, lh_launch_text(status));
         return -1;
     }
     return 0;
+}
+
+static int launched_ok(const char* what)
+{
+    return launched((int)hipGetLastError(), what);
 }
 
 // Token stride of the MFMA scratch: whole 128-token tiles, so every
@@ -1032,18 +1036,16 @@ static int layer_small(const lh_layer_weights* w, float* d_x, float* d_keys, flo
     float* scale_b = group_scales(ws);
     if ((!input_split &&
             residual_norm_split(NULL, 0, T, 1.0f, d_x, w->input_norm, xs, NULL, n, s)) ||
-        lh_launch_small_qkv(w->qkv, w->scale[0], w->scale[1], w->scale[2], xs, T, ws->d_params, n,
-            ws->d_q, d_keys, d_values, C, s) ||
-        launched_ok("qkv") ||
-        lh_launch_attention_mfma(ws->d_q, d_keys, d_values, ws->d_params, (uint32_t)ws->length,
-            n, C, ws->d_PM, ws->d_PT, ws->d_PA, ws->d_attn, xs, T, scale_b, s) ||
-        launched_ok("attention") ||
-        lh_launch_small_o(w->o, w->scale[3], xs, T, scale_b, n, d_x, s) || launched_ok("o") ||
+        launched(lh_launch_small_qkv(w->qkv, w->scale[0], w->scale[1], w->scale[2], xs, T,
+            ws->d_params, n, ws->d_q, d_keys, d_values, C, s), "qkv") ||
+        launched(lh_launch_attention_mfma(ws->d_q, d_keys, d_values, ws->d_params,
+            (uint32_t)ws->length, n, C, ws->d_PM, ws->d_PT, ws->d_PA, ws->d_attn, xs, T, scale_b,
+            s), "attention") ||
+        launched(lh_launch_small_o(w->o, w->scale[3], xs, T, scale_b, n, d_x, s), "o") ||
         residual_norm_split(NULL, 0, T, 1.0f, d_x, w->post_norm, xs, scale_a, n, s) ||
-        lh_launch_small_gateup(w->gate, w->up, w->scale[4], w->scale[5], xs, T, scale_a, n, xd,
-            s) ||
-        launched_ok("gate/up") ||
-        lh_launch_small_down(w->down, w->scale[6], xd, T, n, d_x, s) || launched_ok("down")) {
+        launched(lh_launch_small_gateup(w->gate, w->up, w->scale[4], w->scale[5], xs, T, scale_a,
+            n, xd, s), "gate/up") ||
+        launched(lh_launch_small_down(w->down, w->scale[6], xd, T, n, d_x, s), "down")) {
         return -1;
     }
     return next_norm ? residual_norm_split(NULL, 0, T, 1.0f, d_x, next_norm, xs, NULL, n, s) : 0;
@@ -1101,9 +1103,9 @@ extern "C" int lh_layer_forward_mfma(const lh_layer_weights* w, float* d_x, floa
     // scales back. o: 3072 rows, 4096 columns; residual, post-norm and the
     // gate|up input after it.
     const uint32_t so = LH_KV_HEADS;
-    if (lh_launch_attention_mfma(ws->d_q, d_keys, d_values, ws->d_params, (uint32_t)ws->length,
-            n, C, ws->d_PM, ws->d_PT, ws->d_PA, ws->d_attn, xs, B, scale_b, s) ||
-        launched_ok("attention") ||
+    if (launched(lh_launch_attention_mfma(ws->d_q, d_keys, d_values, ws->d_params,
+            (uint32_t)ws->length, n, C, ws->d_PM, ws->d_PT, ws->d_PA, ws->d_attn, xs, B, scale_b,
+            s), "attention") ||
         gemm(PLANES_F16, w->o, NULL, LH_HIDDEN, LH_HIDDEN, LH_QUERY, xs, B, n, so, P, s, 3,
             scale_b, LH_KV_HEADS) ||
         residual_norm_split(P, so, B, w->scale[3], d_x, w->post_norm, xs, scale_a, n, s)) {

@@ -273,7 +273,7 @@ static int launch_small(const SmallArgs& a, hipStream_t s)
         hipLaunchKernelGGL((k_small<K, P, 2, NR, DEPTH2, EPI>), dim3(SMALL_GROUPS), dim3(512), 0,
             s, a);
     }
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }
 
 extern "C" int lh_launch_small_qkv(const uint8_t* W, float sq, float sk, float sv,

@@ -140,14 +140,14 @@ extern "C" int lh_launch_element(int mode, const float* a, const float* b, float
     hipStream_t s)
 {
     hipLaunchKernelGGL(k_element, grid_for(n), dim3(256), 0, s, mode, a, b, out, n);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }
 
 extern "C" int lh_launch_silu_mul(const float* gate, const float* up, float* out, size_t n,
     hipStream_t s)
 {
     hipLaunchKernelGGL(k_silu_mul, grid_for(n), dim3(256), 0, s, gate, up, out, n);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }
 
 extern "C" int lh_launch_rope(const float* x, const float* cosine, const float* sine,
@@ -155,7 +155,7 @@ extern "C" int lh_launch_rope(const float* x, const float* cosine, const float* 
 {
     hipLaunchKernelGGL(k_rope, grid_for((size_t)width * tokens), dim3(256), 0, s, x, cosine, sine,
         qfactor, out, width, tokens);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }
 
 extern "C" int lh_launch_rope_append(const float* q_raw, const float* k_raw, const float* v_raw,
@@ -164,19 +164,19 @@ extern "C" int lh_launch_rope_append(const float* q_raw, const float* k_raw, con
 {
     hipLaunchKernelGGL(k_rope_append, dim3(count), dim3(256), 0, s, q_raw, k_raw, v_raw, params,
         q, kcache_layer, vcache_layer, capacity);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }
 
 extern "C" int lh_launch_fp8_decode(const uint8_t* codes, float* out, size_t n, hipStream_t s)
 {
     hipLaunchKernelGGL(k_fp8_decode, grid_for(n), dim3(256), 0, s, codes, out, n);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }
 
 extern "C" int lh_launch_expf(const float* x, float* out, size_t n, hipStream_t s)
 {
     hipLaunchKernelGGL(k_expf, grid_for(n), dim3(256), 0, s, x, out, n);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }
 
 extern "C" int lh_launch_read_floor(const void* src, size_t bytes, uint32_t grid, uint32_t unroll,
@@ -191,5 +191,5 @@ extern "C" int lh_launch_read_floor(const void* src, size_t bytes, uint32_t grid
     case 8: hipLaunchKernelGGL(k_read_floor<8>, dim3(grid), dim3(256), 0, s, w, words, sink); break;
     default: return -1;
     }
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }

@@ -438,12 +438,12 @@ extern "C" int lh_launch_paged_append(const lh_paged_cache* cache, const lh_page
     const lh_append_rows* rows, hipStream_t s)
 {
     LH_FOR_CACHE(cache, append, cache, batch, rows, s);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }
 
 extern "C" int lh_launch_paged_read(const lh_paged_cache* cache, const lh_paged_batch* batch,
     float* keys, size_t k_stride, float* values, size_t v_stride, hipStream_t s)
 {
     LH_FOR_CACHE(cache, read, cache, batch, keys, k_stride, values, v_stride, s);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }

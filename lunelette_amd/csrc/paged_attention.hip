@@ -1410,5 +1410,5 @@ extern "C" int lh_launch_paged_attention(const lh_paged_cache* cache, const lh_p
         (((uint64_t)1 << 32) + in_page - 1) / in_page, scale * 1.44269504088896341f, group,
         p.splits, p.tiles, p.chunk, p.tile};
     LH_FOR_CACHE(cache, attention, cache, batch, p, a, s);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }

@@ -796,7 +796,7 @@ using namespace lh;
 
 static int launched()
 {
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }
 
 // One token tile per workgroup: two workgroups fit a CU (128 registers, at most

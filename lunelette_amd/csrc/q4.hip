@@ -796,7 +796,7 @@ extern "C" int lh_launch_q4_pack(const uint8_t* codes, const uint16_t* scales, u
     const Q4Shape p = q4_shape(rows, cols, group);
     hipLaunchKernelGGL(k_q4_pack, dim3(p.tiles, p.blocks), dim3(256), 0, s, codes, scales, p,
         packed);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }
 
 extern "C" int lh_launch_q4_quantize(const float* w, uint32_t rows, uint32_t cols, uint32_t group,
@@ -804,7 +804,7 @@ extern "C" int lh_launch_q4_quantize(const float* w, uint32_t rows, uint32_t col
 {
     const Q4Shape p = q4_shape(rows, cols, group);
     hipLaunchKernelGGL(k_q4_quantize, dim3(p.tiles, p.blocks), dim3(256), 0, s, w, p, packed);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }
 
 // How a product runs: few tokens, some, or many. rt row tiles a workgroup of
@@ -945,8 +945,8 @@ extern "C" int lh_launch_q4_matvec(const uint8_t* packed, const float* x, size_t
         planes, factors, reinterpret_cast<float*>(scratch + p.planes + p.factors)};
     if (p.way == Q4_MANY) {
         hipLaunchKernelGGL(k_q4_planes, dim3(tokens), dim3(1024), 0, s, a, planes, factors);
-        if (hipGetLastError() != hipSuccess) {
-            return -1;
+        if (const hipError_t e = hipGetLastError()) {
+            return (int)e;
         }
     }
     switch (group) {
@@ -954,12 +954,12 @@ extern "C" int lh_launch_q4_matvec(const uint8_t* packed, const float* x, size_t
     case 64: q4_product<2>(p, a, s); break;
     default: q4_product<1>(p, a, s); break;
     }
-    if (hipGetLastError() != hipSuccess) {
-        return -1;
+    if (const hipError_t e = hipGetLastError()) {
+        return (int)e;
     }
     if (p.splits > 1) {
         hipLaunchKernelGGL(k_q4_join, dim3((rows + 255) / 256, tokens), dim3(256), 0, s, a,
             p.splits);
     }
-    return hipGetLastError() == hipSuccess ? 0 : -1;
+    return (int)hipGetLastError();
 }
