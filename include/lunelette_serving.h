@@ -45,8 +45,8 @@ size_t lh_q4_scratch(size_t cols, size_t tokens);
  * x_stride and y_stride elements apart (x_stride >= cols, y_stride >= rows).
  * Products are formed from x as two FP16 planes scaled by a power of two per
  * token, or per token and 128 columns (each x to 2^-22 of itself or 2^-38 of
- * its row's largest), sums are FP32. A row of x with an Inf or NaN gives NaN in
- * its row of y. y must not overlap x. */
+ * its row's largest), sums are FP32, which scales below 2^102 stay in. A row of x
+ * with an Inf or NaN gives NaN in its row of y. y must not overlap x. */
 int lh_q4_matvec(const void *d_packed, const float *d_x, size_t x_stride, float *d_y,
     size_t y_stride, size_t rows, size_t cols, size_t group, size_t tokens, void *d_scratch,
     size_t scratch_bytes, void *stream);

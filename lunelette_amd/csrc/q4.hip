@@ -247,8 +247,9 @@ __device__ __forceinline__ void q4_multiply_block(const Q4Block<PER, RT>& b, con
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     if constexpr (PER * RT * NT > 24) {
-                        // No registers for a block's sums.
-                        acc[t][n][i] = __builtin_fmaf(s[i] * f[n], d[t][n][i], acc[t][n][i]);
+                        // No registers for a block's sums. (The scale meets the sum first, as
+                        // below: with f it may leave FP32's range where the sum is 0.)
+                        acc[t][n][i] = __builtin_fmaf(s[i] * d[t][n][i], f[n], acc[t][n][i]);
                         continue;
                     }
                     sum[t][n][i] = j < STEPS ? s[i] * d[t][n][i]

@@ -181,3 +181,20 @@ def test_paged_ends_of_the_scale(gpu, kind, dim, heads, count, prefix, size, sca
     for t in range(count):
         want, off = so.attention(q[t], keys, values, 70 + prefix + t, scale)
         close(got[t], want, off)
+
+
+@pytest.mark.parametrize("tokens", [1, 8, 16, 40, 64, 100])
+@pytest.mark.parametrize("group", [32, 128])
+def test_q4_matvec_large_beside_zero_weights(gpu, group, tokens):
+    """Weights of 0 (code 8) with large scales under large x: nothing of them in y,
+    which holds what the other 128-column blocks give."""
+    rows, cols = 48, 512
+    rng = np.random.default_rng(tokens)
+    codes, scales = so.q4_random(rng, rows, cols, group)
+    codes[:, 128:256] = 8
+    scales[:, 128 // group:256 // group] = so.bf16(np.float32(1e16))
+    x = rng.normal(size=(tokens, cols)).astype(np.float32)
+    x[:, 128:256] *= np.float32(1e30)
+    w = so.q4_weights(codes, scales, group)
+    got = so.q4_run(gpu, so.q4_on_device(gpu, codes, scales, group), x, rows, cols, group)
+    close(got, x.astype(np.float64) @ w.T, so.q4_bound(w, x))
