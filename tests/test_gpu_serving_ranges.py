@@ -198,3 +198,110 @@ def test_q4_matvec_large_beside_zero_weights(gpu, group, tokens):
     w = so.q4_weights(codes, scales, group)
     got = so.q4_run(gpu, so.q4_on_device(gpu, codes, scales, group), x, rows, cols, group)
     close(got, x.astype(np.float64) @ w.T, so.q4_bound(w, x))
+
+
+@pytest.mark.parametrize("rows,cols,group,tokens", [
+    (200, 8320, 64, 129), (90, 16640, 128, 140), (61, 20608, 32, 150), (2051, 1088, 64, 200),
+    (700, 2176, 128, 131), (8300, 640, 128, 70), (8300, 576, 64, 128), (33, 65536, 128, 129)])
+def test_q4_matvec_many_tokens(gpu, rows, cols, group, tokens):
+    """Products whose planes a launch of their own makes: every group size, ragged
+    token tiles, column splits, rows of x past what a thread of that launch holds."""
+    rng = np.random.default_rng(rows + tokens)
+    codes, scales = so.q4_random(rng, rows, cols, group)
+    x = (rng.normal(size=(tokens, cols)) * np.exp(rng.normal(size=cols))).astype(np.float32)
+    w = so.q4_weights(codes, scales, group)
+    packed = so.q4_on_device(gpu, codes, scales, group)
+    got = so.q4_run(gpu, packed, x, rows, cols, group, x_pad=3, y_pad=1)
+    close(got, x.astype(np.float64) @ w.T, so.q4_bound(w, x))
+
+
+@pytest.mark.parametrize("rows,tokens", [(48, 100), (48, 130), (8300, 70)])
+def test_q4_matvec_special_rows_of_many(gpu, rows, tokens):
+    """Rows of every magnitude, a zero row, and rows with an Inf or NaN, which stay
+    their own row's, past 64 tokens."""
+    cols, group = 384, 64
+    rng = np.random.default_rng(tokens)
+    codes, scales = so.q4_random(rng, rows, cols, group)
+    x = rng.normal(size=(tokens, cols)).astype(np.float32)
+    for first in (0, 50, tokens - 6):
+        x[first] = 0
+        x[first + 1] *= np.float32(1e36)
+        x[first + 2] *= np.float32(1e-36)
+        x[first + 3, 100] = -np.inf
+        x[first + 4, 383] = np.nan
+        x[first + 5, 11] = 1e5
+    packed = so.q4_on_device(gpu, codes, scales, group)
+    w = so.q4_weights(codes, scales, group)
+    got = so.q4_run(gpu, packed, x, rows, cols, group)
+    odd = ~np.isfinite(x).all(1)
+    x = np.where(np.isfinite(x), x, 0)
+    want = x.astype(np.float64) @ w.T
+    want[odd] = np.nan
+    # Elements below 2^-16 of their row's largest carry 2^-38 of that instead.
+    bound = so.q4_bound(w, x) + np.abs(w).sum(1) * 2.0 ** -38 * np.abs(x).max(
+        1, keepdims=True).astype(np.float64)
+    close(got, want, bound)
+
+
+@pytest.mark.parametrize("tokens", [1, 9, 16, 40, 100, 130])
+def test_q4_matvec_planes_of_single_columns(gpu, tokens):
+    """Rows with one weight each, x of every size down to 2^-40 of the token's
+    largest: each element by itself to 2^-22 of itself or 2^-38 of the largest."""
+    rows, cols, group = 256, 640, 32
+    rng = np.random.default_rng(tokens)
+    codes = np.full((rows, cols), 8, np.uint8)
+    at = rng.integers(0, cols, size=rows)
+    codes[np.arange(rows), at] = rng.choice(np.uint8([0, 1, 7, 9, 15]), size=rows)
+    scales = so.bf16(rng.uniform(0.5, 2.0, size=(rows, cols // group)))
+    x = np.ldexp(rng.normal(size=(tokens, cols)), rng.integers(-40, 1, size=(tokens, cols)))
+    x = x.astype(np.float32)
+    x[:, 3] = 1
+    w = so.q4_weights(codes, scales, group)
+    got = so.q4_run(gpu, so.q4_on_device(gpu, codes, scales, group), x, rows, cols, group)
+    largest = np.abs(x).max(1, keepdims=True).astype(np.float64)
+    one = np.abs(x).astype(np.float64)[:, at]
+    # Two products, the group's scale and the power of two back: five roundings.
+    off = np.maximum(one * 2.0 ** -22, largest * 2.0 ** -38) + 5 * so.EPS32 * one
+    close(got, x.astype(np.float64) @ w.T, off * np.abs(w).max(1))
+
+
+@pytest.mark.parametrize("group", [64, 128])
+def test_q4_quantize_groups(gpu, group):
+    """Rounded weights with the larger groups and columns that end inside a block."""
+    rows, cols = 35, 3 * group
+    rng = np.random.default_rng(group)
+    w = rng.normal(size=(rows, cols)).astype(np.float32)
+    w[3, :group] = 0
+    w[5, group + 3] = -np.inf
+    w[6] *= np.float32(1e30)
+    w[7, :group] = np.float32(1e-44)
+    blocks = w.reshape(rows, -1, group)
+    with np.errstate(invalid="ignore", divide="ignore"):
+        scales = so.bf16(np.abs(blocks).max(-1) / np.float32(7))
+        scales[~np.isfinite(blocks).all(-1)] = np.nan
+        code = np.rint(np.clip(blocks / scales[..., None], -7, 7))
+    code = np.where(scales[..., None] > 0, code, 0.0)
+    want = (code * scales[..., None]).reshape(rows, cols)
+    packed = lh.DeviceBuffer(gpu.lh_q4_bytes(rows, cols, group))
+    d_w = lh.DeviceBuffer.from_array(w)
+    lh.check(gpu.lh_q4_quantize(d_w.ptr, rows, cols, group, packed.ptr, None))
+    got = so.q4_run(gpu, packed, np.eye(cols, dtype=np.float32), rows, cols, group).T
+    odd = np.isnan(want).any(1)
+    assert list(np.nonzero(odd)[0]) == [5]
+    assert np.array_equal(got[~odd], want[~odd].astype(np.float32))
+    assert np.isnan(got[5]).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,heads,count", [(64, 2, 1), (128, 1, 3)])
+def test_paged_most_splits(gpu, kind, dim, heads, count):
+    """As many splits as one token's attention is ever cut into."""
+    n = 133003
+    rng = np.random.default_rng(dim)
+    k, v = (rng.normal(size=(n, dim)).astype(np.float32) for _ in range(2))
+    seq, keys, values = filled(gpu, kind, dim, heads, k, v, page=256)
+    q = rng.normal(size=(count, heads, dim)).astype(np.float32)
+    got = seq.attention(seq.batch([count], [n]), q, 0.125)
+    for t in range(count):
+        want, off = so.attention(q[t], keys, values, n - count + t, 0.125)
+        close(got[t], want, off)
