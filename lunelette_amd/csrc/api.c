@@ -23,9 +23,12 @@ const char *lh_last_error(void)
     return last_error;
 }
 
+/* An error that a call reports is taken off the runtime's record, here and in the
+ * allocations below: a launch asks that record for its own status. */
 static int ok(hipError_t status, const char *what)
 {
     if (status != hipSuccess) {
+        (void)hipGetLastError();
         lh_set_error("%s: %s", what, hipGetErrorString(status));
         return -1;
     }
@@ -74,6 +77,7 @@ hipError_t lh_dev_malloc(void **ptr, size_t bytes)
     if (status == hipSuccess) {
         count_live(1);
     } else {
+        (void)hipGetLastError();
         *ptr = NULL;
     }
     return status;
@@ -89,6 +93,7 @@ hipError_t lh_host_malloc(void **ptr, size_t bytes, unsigned flags)
     if (status == hipSuccess) {
         count_live(1);
     } else {
+        (void)hipGetLastError();
         *ptr = NULL;
     }
     return status;

@@ -11,6 +11,7 @@
 static int check(hipError_t status, const char *what)
 {
     if (status != hipSuccess) {
+        (void)hipGetLastError();   /* reported here: not the next launch's */
         lh_set_error("%s: %s", what, hipGetErrorString(status));
         return -1;
     }

@@ -146,6 +146,7 @@ static void destroy_runtime(lh_runtime *rt)
 static int hip_ok(hipError_t status, const char *what, char *error, size_t capacity)
 {
     if (status != hipSuccess) {
+        (void)hipGetLastError();   /* reported here: not the next launch's */
         if (error && capacity) {
             snprintf(error, capacity, "HIP %s failed: %s", what, hipGetErrorString(status));
         }

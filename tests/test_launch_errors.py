@@ -8,8 +8,26 @@ import sys
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 SHIM = r"""
-/* Every launch fails with hipErrorInvalidConfiguration, recorded as the runtime does. */
+/* Every launch fails with hipErrorInvalidConfiguration, or none does, allocations and
+ * waits with hipErrorOutOfMemory; recorded as the runtime does. */
+#include <stddef.h>
 static __thread int last;
+int launch_status = 9;
+int hipMalloc(void **p, size_t n)
+{
+    (void)n;
+    *p = NULL;
+    return last = 2;
+}
+int hipHostMalloc(void **p, size_t n, unsigned flags)
+{
+    (void)flags;
+    return hipMalloc(p, n);
+}
+int hipDeviceSynchronize(void)
+{
+    return last = 2;
+}
 int __hipPushCallConfiguration(void)
 {
     return 0;
@@ -21,7 +39,10 @@ int __hipPopCallConfiguration(void)
 int hipLaunchKernel(const void *f, ...)
 {
     (void)f;
-    return last = 9;
+    if (launch_status) {
+        last = launch_status;
+    }
+    return launch_status;
 }
 int hipGetLastError(void)
 {
@@ -67,16 +88,40 @@ for name, call in calls.items():
         print(name.strip(), "|", call(), "|", lh.last_error(), flush=True)
 """
 
+AFTER = r"""
+import ctypes, sys
+shim = ctypes.CDLL(sys.argv[1], mode=ctypes.RTLD_GLOBAL)
+import lunelette_amd as lh
+l = lh.lib()
+P = 0x10000
+ctypes.c_int.in_dll(shim, "launch_status").value = 0
+for fail in (lambda: l.lh_device_alloc(64) is None, lambda: l.lh_host_alloc_pinned(64) is None,
+             lambda: l.lh_device_synchronize() == -1):
+    print(fail(), "out of memory" in lh.last_error(), l.lh_q4_pack(P, P, 16, 64, 64, P, None),
+          l.lh_rmsnorm(P, P, 2 * P, 64, 1, None), flush=True)
+"""
 
-def test_refused_launches_keep_the_runtimes_words(tmp_path):
+
+def run(tmp_path, program):
+    """The lines that a program prints with the answering library loaded first."""
     source, shim = tmp_path / "shim.c", tmp_path / "libshim.so"
     source.write_text(SHIM)
     subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(shim), str(source)], check=True)
-    out = subprocess.run([sys.executable, "-c", CHILD, str(shim)], cwd=ROOT, text=True,
+    out = subprocess.run([sys.executable, "-c", program, str(shim)], cwd=ROOT, text=True,
                          stdout=subprocess.PIPE, stderr=subprocess.PIPE, timeout=300)
     assert out.returncode == 0, out.stderr
-    lines = [line.split(" | ") for line in out.stdout.splitlines()]
+    return out.stdout.splitlines()
+
+
+def test_refused_launches_keep_the_runtimes_words(tmp_path):
+    lines = [line.split(" | ") for line in run(tmp_path, CHILD)]
     assert len(lines) == 20
     for name, status, text in lines:
         assert status == "-1", name
         assert name in text and "invalid configuration" in text, (name, text)
+
+
+def test_reported_errors_are_not_the_next_launches(tmp_path):
+    """An allocation or wait that failed and said so leaves the next launch its own
+    status."""
+    assert run(tmp_path, AFTER) == ["True True 0 0"] * 3
