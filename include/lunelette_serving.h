@@ -39,7 +39,8 @@ int lh_q4_pack(const uint8_t *d_codes, const uint16_t *d_scales, size_t rows, si
  * zero has code 8 everywhere; one with a nonfinite weight a NaN scale. */
 int lh_q4_quantize(const float *d_w, size_t rows, size_t cols, size_t group, void *d_packed,
     void *stream);
-/* Scratch bytes of lh_q4_matvec at these sizes (0: none is needed). */
+/* Scratch bytes of lh_q4_matvec at these sizes for any number of rows (0: none is
+ * needed). */
 size_t lh_q4_scratch(size_t cols, size_t tokens);
 /* y[t][r] = sum_c w[r][c] x[t][c] for 1..65535 tokens; rows of x and y are
  * x_stride and y_stride elements apart (x_stride >= cols, y_stride >= rows).
@@ -121,7 +122,7 @@ typedef struct {
  * d_q_out (which may be d_q with the same stride, and otherwise shares no element
  * with another tensor).
  * heads is a multiple of kv_heads up to 64 of them each; 0 leaves the queries
- * out. d_cos and d_sin NULL: rotated already. The rotation is formed in 64 bits
+ * and d_qfactor out. d_cos and d_sin NULL: rotated already. The rotation is formed in 64 bits
  * and rounded to FP32 (for 4-bit codes not at all) before the cache's format.
  * With d_cos or d_qfactor a token whose position is negative or not below
  * `positions` is not appended and its query row is NaN; without them that holds

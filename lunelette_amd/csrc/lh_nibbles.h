@@ -39,7 +39,10 @@ __device__ __forceinline__ f16x8 codes_minus8(uint32_t w, const NibbleMasks& mas
     return __builtin_bit_cast(f16x8, r);
 }
 
-// a and b as two pairs of FP16 planes: hi nearest, lo nearest to the rest. The rest
+// a and b as two pairs of FP16 planes: hi nearest, lo nearest to the rest. Planes of small
+// values are subnormal halves, which the matrix instructions take: they align a sum as if
+// such an operand were 2^-14, so 32 products of subnormal and common numbers come out to
+// 2^-33 (measured), where the largest of a row's planes stand at 2^14. The rest
 // has to be that of the hi which goes into the product: left to itself the compiler
 // forms one by a fused multiplication and conversion and the other from the rounded
 // product, and the two differ by a whole step at a tie (1 of 2^13 values). The asm

@@ -45,8 +45,8 @@ __device__ __forceinline__ float column_sum(float v)
 
 // The reference of a column's softmax need not be its maximum: it follows once that is
 // SLACK (in powers of two) above, so the sums are seldom rescaled (with every new
-// maximum some column of a wave had one in most blocks: 62.6 against 57.1 us for 256
-// tokens after 4096 positions). Probabilities are formed relative to 2^SLACK times the
+// maximum some column of a wave has one in most blocks: 59.5 against 56.3 us for 256
+// tokens after 4096 positions in 4-bit pages). Probabilities are formed relative to 2^SLACK times the
 // reference and stay up to 1 (and a rounding).
 //
 // The second product takes them (in 4-bit pages times their positions' value scales) times
@@ -388,8 +388,9 @@ enum { PROMPT_ROWS = 128 };
 // next one is decoded into the other buffer and the one after is on its way.
 // Of 4-bit pages two teams of four waves take every second block of a split for the same
 // rows and meet in LDS at its end, which halves the parts that splits leave in memory (256
-// tokens after 4096: 57.1 us, with one team and twice the splits 60.6; 64 tokens 32 and
-// 36). FP16 pages wait for the other team's loads too then (57.2 against 53.5).
+// tokens after 4096: 56.3 us, with one team and twice the workgroups 59.1; 64 tokens 30.8
+// and 36.3). FP16 pages wait for the other team's loads too then (256 tokens: 56.5
+// against 54.5, though 64 tokens 31.6 against 35.9).
 template <bool Q4>
 constexpr int TEAMS = Q4 ? 2 : 1;
 
@@ -1310,15 +1311,18 @@ k_paged_join(AttentionArgs a)
 
 using namespace lh;
 
-// How the steps are split. RESIDENT workgroups are on the chip at once; up to them a
-// split takes as few as MIN_CHUNK steps (one sequence of 16000 positions: 13.7 us with
-// 8, 15.4 with 4, 14.7 with 12). Past them FULL_CHUNK at least, which pays for a
-// workgroup's start (32 sequences up to 4352 in FP16: 30 us with 12 or 16, 33 with 24), and about
-// WORKGROUPS in all, so that sequences of other lengths than the bound spread evenly
-// (64 up to 17920 in 4 bits: 102 us with 1024, 103 with 2048, 127 with 512, 122 with 8192).
+// How the steps are split. RESIDENT workgroups of the tiles of 4 and 8 rows are on the chip
+// at once (of the tiles of 16 rows of 128 dims, one wave a SIMD, half as many, which the
+// plan does not go by); up to them a split takes as few as MIN_CHUNK steps (one sequence
+// of 15999 positions: 13.9 us with 8, 16.5 with 4, 15.2 with 12). Past them FULL_CHUNK at
+// least, which pays for a workgroup's start (32 sequences up to 4352 in FP16: 36.1 us,
+// with 12 36.5, with 24 44.1), and about WORKGROUPS in all, so that sequences of other
+// lengths than the bound spread evenly (64 up to 17920 in 4 bits: 102 us with 2048, 99
+// with 1024, 121 with 512, 118 with 8192; in FP16 285, 328, 313 and 289).
 // A prompt's workgroup (team) has 128 rows, and the splits' parts are as large as its
-// output for each: PROMPT_WORKGROUPS teams in all (256 tokens after 4096 positions, one
-// team a workgroup: 57 us with 512, 68 with 256, 118 with 128), PROMPT_CHUNK steps at least.
+// output for each: PROMPT_WORKGROUPS teams in all (256 tokens after 4096 positions in 4-bit
+// pages: 56.3 us with 512, 86.6 with 256, 70.0 with 1024; FP16 54.5, 61.4 and 76.1),
+// PROMPT_CHUNK steps at least.
 enum { RESIDENT = 512, WORKGROUPS = 2048, MIN_CHUNK = 8, FULL_CHUNK = 16,
     PROMPT_WORKGROUPS = 512, PROMPT_CHUNK = 4 };
 
@@ -1332,9 +1336,10 @@ static AttentionPlan attention_plan(const lh_paged_cache* c, const lh_paged_batc
     const uint64_t query = b->max_query < b->tokens ? b->max_query : b->tokens;
     const uint64_t rows = query * group;
     AttentionPlan p;
-    // The least tile that has all rows of a sequence, to 32 (8 sequences up to 4352 in 4
-    // bits and in FP16, group 4: 4 tokens take 29 and 32 us, the prompts' 46 and 42; 8 take
-    // 34 and 36 against 47 and 43; 16 take 50 and 51 against 49 and 45).
+    // The least tile that has all rows of a sequence, to 32 (8 sequences of 500 to 4352 in 4
+    // bits and in FP16, group 4: up to 4 tokens each take 28.5 and 33.3 us, with the
+    // prompts' tile 47.8 and 43.5; up to 8 take 33.9 and 37.5 against 48.2 and 43.9; up to
+    // 16 take 48.3 and 53.5 with tiles of 16 rows, 49.5 and 45.8 with the prompts').
     p.tile = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 32 ? 16 : PROMPT_ROWS;
     const uint64_t tiles = (rows + p.tile - 1) / p.tile;
     p.tiles = (uint32_t)(tiles < 1024 ? tiles : 1024);
