@@ -122,8 +122,9 @@ typedef struct {
  * d_q_out (which may be d_q with the same stride, and otherwise shares no element
  * with another tensor).
  * heads is a multiple of kv_heads up to 64 of them each; 0 leaves the queries
- * and d_qfactor out. d_cos and d_sin NULL: rotated already. The rotation is formed in 64 bits
- * and rounded to FP32 (for 4-bit codes not at all) before the cache's format.
+ * and d_qfactor out. d_cos and d_sin NULL: rotated already. The rotation is formed
+ * in 64 bits and rounded to FP32 (for 4-bit codes not at all) before the cache's
+ * format.
  * With d_cos or d_qfactor a token whose position is negative or not below
  * `positions` is not appended and its query row is NaN; without them that holds
  * for negative positions. A page that a call appends to must stand in one place
@@ -147,10 +148,11 @@ size_t lh_paged_attention_scratch(const lh_paged_cache *cache, const lh_paged_ba
  * gives NaN, as does one that sees a key with an Inf or NaN, or a value with one
  * (in FP16 pages in that element alone). What no token sees may hold anything.
  * Products are formed from two FP16 planes: of queries, which keep them to 2^-22
- * of themselves or 2^-38 of their row's largest, and of probabilities (in 4-bit pages
- * times their values' scales), 2^-22 of themselves or 2^-32 of the row's largest of
- * these. Sums and the softmax are FP32: scores, and a row's number of positions
- * times its largest value, have to lie in its range. */
+ * of themselves or 2^-38 of their row's largest, and of probabilities (in 4-bit
+ * pages times their values' scales), 2^-22 of themselves or 2^-32 of the row's
+ * largest of these. Sums and the softmax are FP32: scores, and a row's number of
+ * positions times its largest value, have to lie in its range. 4-bit keys count to
+ * 2^-125. */
 int lh_paged_attention(const lh_paged_cache *cache, const lh_paged_batch *batch, uint32_t heads,
     const float *d_q, size_t q_stride, float scale, float *d_out, size_t out_stride,
     void *d_scratch, size_t scratch_bytes, void *stream);

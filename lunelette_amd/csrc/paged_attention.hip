@@ -126,7 +126,8 @@ __device__ __forceinline__ void load_query(const float* q, uint32_t g, float sca
     for (int e = 0; e < D / 4; e++) {
         most = fmaxf(most, fabsf(v[e]));
     }
-    const int e2 = row_exponent(column_max(most));
+    most = column_max(most);
+    const int e2 = row_exponent(most);
     const float up = exp2i(e2);
 #pragma unroll
     for (int e = 0; e < D / 4; e++) {
@@ -144,8 +145,9 @@ __device__ __forceinline__ void load_query(const float* q, uint32_t g, float sca
     qs = column_sum(sum);
     // Never 0 or Inf, which a hidden or a zero score would turn into NaN. Scores of FP16 keys
     // are below 2^39, so they vanish before cs does; 4-bit keys reach 2^128 and meet cs (to
-    // 2^-150), or KEY_UNIT, before the sums, so that any score that FP32 holds is formed.
-    cs = fminf(fmaxf(scale * exp2i(-e2), 0x1p-149f), 3e38f);
+    // 2^-150), or KEY_UNIT, before the sums, so that any score that FP32 holds is formed. A
+    // row of zeros takes the least: its planes may be a step each, and the scale is any.
+    cs = most == 0 ? 0x1p-149f : fminf(fmaxf(scale * exp2i(-e2), 0x1p-149f), 3e38f);
 }
 
 // Prompts: four waves with 32 query rows each (two column tiles) share every block of 32

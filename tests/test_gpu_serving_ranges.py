@@ -305,3 +305,22 @@ def test_paged_most_splits(gpu, kind, dim, heads, count):
     for t in range(count):
         want, off = so.attention(q[t], keys, values, n - count + t, 0.125)
         close(got[t], want, off)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,heads,count,prefix", CALLS)
+@pytest.mark.parametrize("scale", [1.0, 1e15, 1e38])
+def test_paged_zero_queries(gpu, kind, dim, heads, count, prefix, scale):
+    """A query of zeros has scores of 0 at any scale: the mean of what it sees."""
+    rng = np.random.default_rng(dim + count)
+    n = 70 + prefix + count
+    k = (rng.normal(size=(n, dim)) * 1e4).astype(np.float32)
+    v = rng.normal(size=(n, dim)).astype(np.float32)
+    seq, keys, values = filled(gpu, kind, dim, heads, k, v)
+    q = np.zeros((count, heads, dim), np.float32)
+    q[::2] = -0.0
+    scale = float(np.float32(scale))
+    got = seq.attention(seq.batch([count], [n]), q, scale)
+    for t in range(count):
+        want, off = so.attention(q[t], keys, values, 70 + prefix + t, scale)
+        close(got[t], want, off)
