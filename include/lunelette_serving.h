@@ -1,7 +1,8 @@
 /* Operators of batched serving from little memory (no counterpart in the
  * reference): a paged KV cache of several sequences in FP16 rows or 4-bit
  * codes with the append and the attention that use it, products with 4-bit
- * weights, and log probabilities of logit rows.
+ * weights, products of 8-bit rows with 8-bit weights, log probabilities of logit
+ * rows, and beam search over both.
  *
  * The conventions are those of lunelette_kernels.h: pointers named d_* are
  * device pointers on the current device, `stream` is a hipStream_t passed as
@@ -51,6 +52,52 @@ size_t lh_q4_scratch(size_t cols, size_t tokens);
 int lh_q4_matvec(const void *d_packed, const float *d_x, size_t x_stride, float *d_y,
     size_t y_stride, size_t rows, size_t cols, size_t group, size_t tokens, void *d_scratch,
     size_t scratch_bytes, void *stream);
+
+/* ---- 8-bit rows and weights ----
+ * 8-bit rows: codes [tokens][width], code_stride bytes apart, of which each row
+ * has an FP32 scale: v[t][c] = scale[t] * code[t][c]. They lie on 16-byte
+ * boundaries, code_stride is a multiple of 16, and the last row has its bytes up
+ * to the next multiple of 16 too; what those past the width hold is not used and
+ * stays. Width 1..65536, 1..65535 tokens, as cols and tokens of the product. */
+
+/* Rounds rows of FP32 values v to 8-bit rows: scale = max |v| / 127 in FP32, code =
+ * rint(v / scale) within -127..127, both from 64-bit values. A row whose scale
+ * rounds to 0 has codes of 0; one with an Inf or NaN, or whose scale overflows, has a
+ * scale of NaN and codes of 0. The codes and scales share no byte with the inputs.
+ * lh_q8_rows: v = x. */
+int lh_q8_rows(const float *d_x, size_t x_stride, size_t width, size_t tokens, int8_t *d_codes,
+    size_t code_stride, float *d_scales, void *stream);
+/* v = SiLU(gate) * up, formed in 64 bits; gate and up may be parts of one
+ * product's rows (one stride). */
+int lh_q8_silu(const float *d_gate, size_t gate_stride, const float *d_up, size_t up_stride,
+    size_t width, size_t tokens, int8_t *d_codes, size_t code_stride, float *d_scales,
+    void *stream);
+/* v = gamma * (h / sqrt(mean(h^2) + 1e-5)), formed in 64 bits from the FP32 sums
+ * h = x + add, which are written to d_sum (the residual of the next addition).
+ * d_add NULL: h = x. d_sum NULL: h is not kept. d_sum may be d_x or d_add, with the
+ * same stride, and otherwise shares no element with another tensor. */
+int lh_q8_norm(const float *d_x, size_t x_stride, const float *d_add, size_t add_stride,
+    const float *d_gamma, float *d_sum, size_t sum_stride, size_t width, size_t tokens,
+    int8_t *d_codes, size_t code_stride, float *d_scales, void *stream);
+
+/* Bytes of packed 8-bit weights w[r][c] = scale[r] * code[r][c] (16-row tiles in the
+ * order in which the matrix instructions take them): rows 1..2^20, cols 1..65536; 0
+ * for other sizes. */
+size_t lh_q8_bytes(size_t rows, size_t cols);
+/* Lays out d_codes [rows][cols] (any int8) and d_scales [rows] as packed weights. */
+int lh_q8_pack(const int8_t *d_codes, const float *d_scales, size_t rows, size_t cols,
+    void *d_packed, void *stream);
+/* Packs d_w [rows][cols] FP32, each row rounded as lh_q8_rows does. */
+int lh_q8_quantize(const float *d_w, size_t rows, size_t cols, void *d_packed, void *stream);
+/* Scratch bytes of lh_q8_matvec (0: none is needed, or sizes that it refuses). */
+size_t lh_q8_scratch(size_t rows, size_t cols, size_t tokens);
+/* y[t][r] = x_scale[t] * (w_scale[r] * sum_c w_code[r][c] x_code[t][c]) for 8-bit
+ * rows d_x: the sums are exact, then FP32 in the order written (three roundings).
+ * A NaN scale gives NaN in its row of y or its column. y_stride >= rows elements;
+ * y shares no byte with the inputs. */
+int lh_q8_matvec(const void *d_packed, const int8_t *d_x, size_t x_stride,
+    const float *d_x_scales, float *d_y, size_t y_stride, size_t rows, size_t cols,
+    size_t tokens, void *d_scratch, size_t scratch_bytes, void *stream);
 
 /* ---- log probabilities ---- */
 
@@ -156,6 +203,53 @@ size_t lh_paged_attention_scratch(const lh_paged_cache *cache, const lh_paged_ba
 int lh_paged_attention(const lh_paged_cache *cache, const lh_paged_batch *batch, uint32_t heads,
     const float *d_q, size_t q_stride, float scale, float *d_out, size_t out_stride,
     void *d_scratch, size_t scratch_bytes, void *stream);
+
+/* ---- beam search ----
+ * Sequence groups * beams of a batch: beam b of group (request) g is row and
+ * sequence g * beams + b. */
+
+#define LH_BEAMS 64   /* of a group, and places that a group keeps */
+
+/* Scratch bytes of lh_beam_select (0: none is needed, or sizes that it refuses). */
+size_t lh_beam_scratch(size_t groups, size_t beams, size_t vocab, size_t keep);
+/* The best continuations of each group's beams. A beam of score s (d_scores
+ * [groups * beams], FP32) has a candidate of score s + ln p for each token of its
+ * row of logits with p = softmax(row); a logit of -Inf is no candidate. A
+ * finished beam (d_done [groups * beams] not 0; NULL: none is) has one, of score s,
+ * with token -1. A beam of score -Inf has none. The logits of the latter two are not
+ * read.
+ * Of each group the best `keep` (1..LH_BEAMS) in falling order of the score in 64 bits,
+ * equal ones by lower beam, then by larger logit, then by lower id: d_parent
+ * [groups][keep] the beam in its group, d_token, d_score (FP32), d_done_out (NULL:
+ * not written) 1 where the parent is finished or the token is `stop` (-1: none).
+ * Places past a group's candidates hold parent -1, token -1, score -Inf, done 0. Where
+ * a beam's score is NaN or +Inf, or the row of one that is read holds a NaN or
+ * +Inf, all places of its group hold parent -1, token -1, score NaN, done 0.
+ * groups * beams 1..65535, beams 1..LH_BEAMS, vocab 1..2^24, stride >= vocab. The
+ * sums are formed in 64 bits. Outputs share no element with inputs. */
+int lh_beam_select(const float *d_logits, size_t stride, size_t groups, size_t beams,
+    size_t vocab, const float *d_scores, const uint8_t *d_done, int64_t stop, size_t keep,
+    int32_t *d_parent, int64_t *d_token, float *d_score, uint8_t *d_done_out, void *d_scratch,
+    size_t scratch_bytes, void *stream);
+/* Makes beam b of each group the continuation of beam d_parent[g][b] ([groups][beams],
+ * as lh_beam_select writes it for keep = beams) in the paged caches of 1..64 layers
+ * (caches[layers] on the host, alike but for d_pages). The beams of a group have one
+ * length: d_length [groups * beams] as in a batch, of which a group's first is read.
+ * Rows of d_table [groups * beams][table_width] become rows of d_table_out (the same
+ * array, or one that shares nothing with it):
+ * - pages before the length's own, which are full, are the parent's and from
+ *   then on shared;
+ * - from the page of position `length` on, which the next append writes, each beam has
+ *   pages of its own: the first child of a parent takes over the parent's, the
+ *   others, in order, those of the beams without children. Where that page is
+ *   begun already, they get a copy of it in every layer.
+ * So no page is allocated, and each of a group's rows must have pages of its own from
+ * there on (rows of beams that never went on, too). A place without a parent (any
+ * other id) is no child and keeps the row of a beam without children. Page
+ * ids outside [0, pages) move with their rows and are not copied. */
+int lh_beam_reorder(const lh_paged_cache *caches, size_t layers, size_t groups, size_t beams,
+    const int32_t *d_parent, const int32_t *d_length, const int32_t *d_table,
+    int32_t *d_table_out, size_t table_width, void *stream);
 
 #ifdef __cplusplus
 }

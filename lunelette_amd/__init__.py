@@ -244,6 +244,14 @@ def declare_serving(l):
     _proto(l, "lh_q4_scratch", c_size, c_size, c_size)
     _proto(l, "lh_q4_matvec", i, p, p, c_size, p, c_size, c_size, c_size, c_size, c_size, p,
            c_size, p)
+    _proto(l, "lh_q8_rows", i, p, c_size, c_size, c_size, p, c_size, p, p)
+    _proto(l, "lh_q8_silu", i, p, c_size, p, c_size, c_size, c_size, p, c_size, p, p)
+    _proto(l, "lh_q8_norm", i, p, c_size, p, c_size, p, p, c_size, c_size, c_size, p, c_size, p, p)
+    _proto(l, "lh_q8_bytes", c_size, c_size, c_size)
+    _proto(l, "lh_q8_pack", i, p, p, c_size, c_size, p, p)
+    _proto(l, "lh_q8_quantize", i, p, c_size, c_size, p, p)
+    _proto(l, "lh_q8_scratch", c_size, c_size, c_size, c_size)
+    _proto(l, "lh_q8_matvec", i, p, p, c_size, p, p, c_size, c_size, c_size, c_size, p, c_size, p)
     _proto(l, "lh_logprobs_scratch", c_size, c_size, c_size, c_size)
     _proto(l, "lh_logprobs", i, p, c_size, c_size, c_size, p, p, p, c_size, p, p, p, c_size, p)
     _proto(l, "lh_paged_cache_bytes", c_size, cache)
@@ -252,6 +260,10 @@ def declare_serving(l):
     _proto(l, "lh_paged_read", i, cache, batch, p, c_size, p, c_size, p)
     _proto(l, "lh_paged_attention_scratch", c_size, cache, batch, u)
     _proto(l, "lh_paged_attention", i, cache, batch, u, p, c_size, f, p, c_size, p, c_size, p)
+    _proto(l, "lh_beam_scratch", c_size, c_size, c_size, c_size, c_size)
+    _proto(l, "lh_beam_select", i, p, c_size, c_size, c_size, c_size, p, p, ctypes.c_int64, c_size,
+           p, p, p, p, p, c_size, p)
+    _proto(l, "lh_beam_reorder", i, cache, c_size, c_size, c_size, p, p, p, p, c_size, p)
 
 
 class SessionWork(ctypes.Structure):
