@@ -87,37 +87,343 @@ struct Q8Args {
     const int8_t* x;
     const float* x_scales;
     float* y;
+    int32_t* part;                  // [split][token][16 tiles] where columns are split
     size_t x_stride, y_stride;
-    uint32_t tokens;
+    uint32_t tokens, splits, per;   // per: 128-column steps of a split
 };
 
-// A wave a tile of 16 rows and 16 tokens.
-__global__ void __launch_bounds__(64)
-k_q8_matvec(Q8Args a)
+// Sums v of rows row .. row + 3 for a token, as y or as a split's part. w: the rows' scales.
+__device__ __forceinline__ void q8_put(const Q8Args& a, float4 w, i32x4 v, uint32_t token,
+    float scale, uint32_t row, uint32_t split)
 {
-    const uint32_t lane = threadIdx.x, tile = blockIdx.x;
-    const uint32_t token = blockIdx.y * 16 + (lane & 15), g = lane >> 4;
-    const uint32_t mine = token < a.tokens ? token : a.tokens - 1;
-    const int8_t* x = a.x + mine * a.x_stride;
-    const i32x4* w = reinterpret_cast<const i32x4*>(a.packed) + (size_t)tile * a.p.blocks * 64;
-    i32x4 acc = {0, 0, 0, 0};
-    for (uint32_t b = 0; b < a.p.blocks; b++) {
-        const uint32_t col = b * 64 + g * 16;
-        // Words past the row's last meet codes of 0.
-        const i32x4 v = *reinterpret_cast<const i32x4*>(x + (col < a.p.cols ? col : 0));
-        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[b * 64 + lane], v, acc, 0, 0, 0);
-    }
-    if (token >= a.tokens) {
+    if (a.splits > 1) {
+        *reinterpret_cast<i32x4*>(a.part + ((size_t)split * a.tokens + token) * (a.p.tiles * 16) +
+            row) = v;
         return;
     }
-    const float scale = a.x_scales[token];
-    const float* ws = q8_scales(a.packed, a.p);
-    for (uint32_t e = 0; e < 4; e++) {
-        const uint32_t row = tile * 16 + 4 * g + e;
-        if (row < a.p.rows) {
-            a.y[token * a.y_stride + row] = scale * (ws[row] * (float)acc[e]);
+    float* y = a.y + token * a.y_stride + row;
+    const float4 r = make_float4(scale * (w.x * (float)v[0]), scale * (w.y * (float)v[1]),
+        scale * (w.z * (float)v[2]), scale * (w.w * (float)v[3]));
+    if (row + 3 < a.p.rows) {
+        store4(y, r);
+        return;
+    }
+    const float e[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 3; i++) {
+        if (row + i < a.p.rows) {
+            y[i] = e[i];
         }
     }
+}
+
+__device__ __forceinline__ float4 q8_row_scales(const Q8Args& a, uint32_t row)
+{
+    return *reinterpret_cast<const float4*>(q8_scales(a.packed, a.p) + row);
+}
+
+// The product of up to 16 tokens. A workgroup takes RT tiles of rows, its eight waves a slice
+// of the columns each; a wave asks for U blocks of its slice at once and for another
+// whenever it has multiplied one. The sums meet in LDS.
+// Bound: the weights' bytes. Measured, cold weights: 18432 x 3072 (57 MB) for one token
+// 10.5 us, 5.4 TB/s, 131072 x 3072 for eight 59 us, 6.8 TB/s; 3072 x 9216 6.8 us, of
+// which a launch and the first bytes' way are 4. Two tiles of rows share the tokens'
+// words where these are 16 rows apart each and there are workgroups enough: 18432 x 3072
+// for 16 tokens 14.0 us (one tile 14.7), 6144 x 3072 for eight 5.7 (6.2); but for one
+// token 11.8 (10.5). More loads on their way (nine blocks) or fewer (three): no gain.
+enum { FEW_WAVES = 8, FEW_BLOCKS = 6 };
+
+template <int RT>
+__global__ void __launch_bounds__(64 * FEW_WAVES)
+k_q8_few(Q8Args a)
+{
+    constexpr int W = FEW_WAVES, U = FEW_BLOCKS;
+    __shared__ i32x4 sums[W][RT][64];
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t tile = blockIdx.x * RT, token = lane & 15;
+    const uint32_t per = (a.p.blocks + W - 1) / W, first = wave * per;
+    const uint32_t end = first + per < a.p.blocks ? first + per : a.p.blocks;
+    const uint32_t last_word = (a.p.cols - 1) & ~15u;
+    const i32x4* w[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        // Tiles past the last repeat it and are not stored.
+        w[t] = reinterpret_cast<const i32x4*>(a.packed) +
+            (size_t)(tile + t < a.p.tiles ? tile + t : a.p.tiles - 1) * a.p.blocks * 64 + lane;
+    }
+    const int8_t* x = a.x + (token < a.tokens ? token : a.tokens - 1) * a.x_stride;
+    i32x4 wr[U][RT], xr[U], acc[RT];
+    auto load = [&](int u, uint32_t b) __attribute__((always_inline)) {
+        // Words past the last column meet codes of 0.
+        const uint32_t col = b * 64 + 16 * (lane >> 4);
+        xr[u] = *reinterpret_cast<const i32x4*>(x + (col < last_word ? col : last_word));
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+            wr[u][t] = __builtin_nontemporal_load(w[t] + (size_t)b * 64);
+        }
+    };
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        if (first + u < end) {
+            load(u, first + u);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        acc[t] = (i32x4){0, 0, 0, 0};
+    }
+    for (uint32_t b = first; b < end; b += U) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (b + u >= end) {
+                break;
+            }
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wr[u][t], xr[u], acc[t], 0, 0, 0);
+            }
+            if (b + u + U < end) {
+                load(u, b + u + U);
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        sums[wave][t][lane] = acc[t];
+    }
+    __syncthreads();
+    if (wave >= RT || token >= a.tokens || tile + wave >= a.p.tiles) {
+        return;
+    }
+    i32x4 v = sums[0][wave][lane];
+#pragma unroll
+    for (int i = 1; i < W; i++) {
+        v += sums[i][wave][lane];
+    }
+    const uint32_t row = (tile + wave) * 16 + 4 * (lane >> 4);
+    q8_put(a, q8_row_scales(a, row), v, token, a.x_scales[token], row, 0);
+}
+
+// The workgroup's barrier after a wait that leaves some of the wave's loads into LDS on
+// their way (__syncthreads waits for all of them).
+template <int WAIT>
+__device__ __forceinline__ void q8_meet()
+{
+    __builtin_amdgcn_s_waitcnt(WAIT);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// The product of many tokens. A workgroup of WM x WN waves forms the sums of MT = WM * MW
+// tiles of rows and NT = WN * NW tiles of tokens, a wave MW x NW of them, over a split
+// of the columns. 128 columns (a step) of both operands at a time go to LDS as they are
+// multiplied, in B buffers: one is multiplied while the others fill.
+// Bound: at large tiles the way of the operands from L2 to LDS beside the matrix
+// instructions: 18432 x 3072 for 2048 tokens takes 117 to 120 us, 1.95e15 operations a
+// second (without the matrix instructions 100). Measured there, too:
+// tiles of 256 x 256 136 us (576 items leave a quarter of the chip idle in their
+// third turn; 8192^3, which they fill, 2.37e15 a second), 128 x 256 in three buffers 147,
+// workgroups that go on to their next item 138 (registers), activations in pieces of 64
+// columns of 16 tokens 134 (half a cache line of each row a request), other starting
+// columns for each workgroup 119 to 124.
+template <int MW, int NW, int WM, int WN, int B>
+__global__ void __launch_bounds__(64 * WM * WN, 2)
+k_q8_tiles(Q8Args a, uint32_t mtiles, uint32_t ntiles)
+{
+    constexpr int W = WM * WN, MT = MW * WM, NT = NW * WN;
+    constexpr int AP = 2 * MT / W, BP = 2 * NT / W;   // 1 KiB pieces a wave fetches
+    static_assert(2 * MT % W == 0 && 2 * NT % W == 0, "pieces are dealt evenly");
+    static_assert((B - 2) * (AP + BP) < 64, "the wait counts pieces");
+    constexpr int SIZE = (MT + NT) * 2048;
+    __shared__ __attribute__((aligned(1024))) uint8_t buf0[SIZE], buf1[SIZE];
+    __shared__ __attribute__((aligned(1024))) uint8_t buf2[B > 2 ? SIZE : 16];
+    __shared__ __attribute__((aligned(1024))) uint8_t buf3[B > 3 ? SIZE : 16];
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t wm = wave % WM, wn = wave / WM;
+    // Neighbouring items to an XCD's workgroups (every eighth): they share rows and tokens
+    // in its L2.
+    uint32_t id = gridDim.x % 8 ? blockIdx.x
+        : (blockIdx.x & 7) * (gridDim.x / 8) + (blockIdx.x >> 3);
+    const uint32_t split = id % a.splits;
+    id /= a.splits;
+    const uint32_t group = ntiles >= 8 ? 4 : 32 / ntiles;
+    const uint32_t base = id / (group * ntiles) * group, in = id % (group * ntiles);
+    const uint32_t rows = mtiles - base < group ? mtiles - base : group;
+    const uint32_t tile0 = (base + in % rows) * MT, token0 = in / rows * (NT * 16);
+    const uint32_t all = (a.p.blocks + 1) / 2, first = split * a.per;
+    const uint32_t end = first + a.per < all ? first + a.per : all;
+    const uint32_t last_word = (a.p.cols - 1) & ~15u;
+    // Where a wave's pieces come from. Of the activations a piece is 128 columns of 8
+    // tokens, a lane's 16-byte word of them turned by its token: so the words that eight
+    // lanes read at once lie in different banks. Tiles and tokens past the last repeat it
+    // and are not stored; words past the last column meet codes of 0.
+    const uint8_t* wfrom[AP];
+    const int8_t* xfrom[BP];
+#pragma unroll
+    for (int n = 0; n < AP; n++) {
+        const uint32_t t = tile0 + (AP * wave + n) / 2;
+        wfrom[n] = a.packed + (size_t)(t < a.p.tiles ? t : a.p.tiles - 1) * a.p.blocks * 1024 +
+            lane * 16;
+    }
+#pragma unroll
+    for (int n = 0; n < BP; n++) {
+        const uint32_t t = token0 + 8 * (BP * wave + n) + (lane >> 3);
+        xfrom[n] = a.x + (t < a.tokens ? t : a.tokens - 1) * a.x_stride;
+    }
+    const uint32_t word = 16 * ((lane & 7) ^ (lane >> 3));
+    // Steps past the last repeat it, so that the number of pieces on their way is the same
+    // at each wait.
+    auto fetch = [&](uint32_t step, uint8_t* to) __attribute__((always_inline)) {
+        step = step < end ? step : end - 1;
+#pragma unroll
+        for (int n = 0; n < AP; n++) {
+            const uint32_t f = AP * wave + n, b = 2 * step + (f & 1);
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void*)(wfrom[n] +
+                    (size_t)(b < a.p.blocks ? b : a.p.blocks - 1) * 1024),
+                (__attribute__((address_space(3))) void*)(to + f * 1024), 16, 0, 0);
+        }
+        const uint32_t col = 128 * step + word;
+#pragma unroll
+        for (int n = 0; n < BP; n++) {
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void*)(xfrom[n] +
+                    (col < last_word ? col : last_word)),
+                (__attribute__((address_space(3))) void*)(to + (2 * MT + BP * wave + n) * 1024), 16,
+                0, 0);
+        }
+    };
+    i32x4 acc[MW][NW];
+#pragma unroll
+    for (int m = 0; m < MW; m++) {
+#pragma unroll
+        for (int n = 0; n < NW; n++) {
+            acc[m][n] = (i32x4){0, 0, 0, 0};
+        }
+    }
+    // A half (64 columns) of a step's operands: of the activations token lane & 15's word
+    // of columns 16 (lane >> 4).
+    const uint32_t x_at = (lane & 15) * 128 + 16 * ((lane >> 4) ^ (lane & 7));
+    auto read = [&](const uint8_t* from, int h, i32x4 (&w)[MW], i32x4 (&x)[NW])
+        __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < NW; n++) {
+            x[n] = *reinterpret_cast<const i32x4*>(from + 2 * (MT + wn * NW + n) * 1024 +
+                (h ? x_at ^ 64 : x_at));
+        }
+#pragma unroll
+        for (int m = 0; m < MW; m++) {
+            w[m] = *reinterpret_cast<const i32x4*>(from + (2 * (wm * MW + m) + h) * 1024 +
+                lane * 16);
+        }
+    };
+    auto multiply = [&](const i32x4 (&w)[MW], const i32x4 (&x)[NW])
+        __attribute__((always_inline)) {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int m = 0; m < MW; m++) {
+#pragma unroll
+            for (int n = 0; n < NW; n++) {
+                acc[m][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[m], x[n], acc[m][n], 0, 0, 0);
+            }
+        }
+        __builtin_amdgcn_s_setprio(0);
+    };
+    // vmcnt(B - 2 steps' pieces), lgkmcnt(0): the next step's pieces, this wave's reads.
+    constexpr int LEFT = (B - 2) * (AP + BP);
+    constexpr int WAIT = 0x0070 | (LEFT & 15) | (LEFT >> 4) << 14;
+    i32x4 w0[MW], x0[NW], w1[MW], x1[NW];
+    // Step s in `now`, whose first half is in registers; the next B - 2 are on their way.
+    auto turn = [&](uint32_t s, uint8_t* now, uint8_t* then) __attribute__((always_inline)) {
+        read(now, 1, w1, x1);
+        multiply(w0, x0);
+        __builtin_amdgcn_sched_barrier(0);
+        q8_meet<WAIT>();
+        fetch(s + B, now);
+        read(then, 0, w0, x0);
+        if (2 * s + 1 < a.p.blocks) {
+            multiply(w1, x1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        return s + 1 < end;
+    };
+    fetch(first, buf0);
+    fetch(first + 1, buf1);
+    if (B > 2) {
+        fetch(first + 2, buf2);
+    }
+    if (B > 3) {
+        fetch(first + 3, buf3);
+    }
+    constexpr int START = (B - 1) * (AP + BP);
+    q8_meet<0x0f70 | (START & 15) | (START >> 4) << 14>();
+    read(buf0, 0, w0, x0);
+    for (uint32_t s = first;; s += B) {
+        if (!turn(s, buf0, buf1)) {
+            break;
+        }
+        if (B == 2) {
+            if (!turn(s + 1, buf1, buf0)) {
+                break;
+            }
+        } else {
+            if (!turn(s + 1, buf1, buf2) || !turn(s + 2, buf2, B > 3 ? buf3 : buf0) ||
+                (B > 3 && !turn(s + 3, buf3, buf0))) {
+                break;
+            }
+        }
+    }
+    // All scales before the first store, behind which the compiler keeps a load.
+    float4 w[MW];
+    float scale[NW];
+#pragma unroll
+    for (int m = 0; m < MW; m++) {
+        const uint32_t t = tile0 + wm * MW + m;
+        w[m] = q8_row_scales(a, (t < a.p.tiles ? t : a.p.tiles - 1) * 16 + 4 * (lane >> 4));
+    }
+#pragma unroll
+    for (int n = 0; n < NW; n++) {
+        const uint32_t token = token0 + (wn * NW + n) * 16 + (lane & 15);
+        scale[n] = a.x_scales[token < a.tokens ? token : a.tokens - 1];
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);   // here: between stores it would wait for those too
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < NW; n++) {
+        const uint32_t token = token0 + (wn * NW + n) * 16 + (lane & 15);
+        if (token >= a.tokens) {
+            continue;
+        }
+#pragma unroll
+        for (int m = 0; m < MW; m++) {
+            const uint32_t tile = tile0 + wm * MW + m;
+            if (tile < a.p.tiles) {
+                q8_put(a, w[m], acc[m][n], token, scale[n], tile * 16 + 4 * (lane >> 4), split);
+            }
+        }
+    }
+}
+
+// Joins the column splits' sums: a thread four rows of a token.
+__global__ void __launch_bounds__(256)
+k_q8_join(Q8Args a)
+{
+    const uint32_t row = (blockIdx.x * 256 + threadIdx.x) * 4, token = blockIdx.y;
+    if (row >= a.p.rows) {
+        return;
+    }
+    const uint32_t splits = a.splits;
+    const size_t wide = a.p.tiles * 16, one = a.tokens * wide;
+    const int32_t* from = a.part + token * wide + row;
+    i32x4 v = *reinterpret_cast<const i32x4*>(from);
+    for (uint32_t i = 1; i < splits; i++) {
+        v += *reinterpret_cast<const i32x4*>(from + i * one);
+    }
+    a.splits = 1;
+    q8_put(a, q8_row_scales(a, row), v, token, a.x_scales[token], row, 0);
 }
 
 }  // namespace lh
@@ -141,16 +447,103 @@ extern "C" int lh_launch_q8_quantize(const float* w, uint32_t rows, uint32_t col
     return (int)hipGetLastError();
 }
 
+// Ways to run a product past 16 tokens: a workgroup's tile, the 1 / 64 us that a step takes
+// it where it is alone on a compute unit, and that it adds where others are there too.
+struct Q8Way {
+    uint32_t rows, tokens, buffers, alone, shared;
+};
+static const Q8Way q8_ways[] = {
+    {64, 32, 4, 14, 11}, {64, 64, 3, 20, 16}, {128, 128, 2, 44, 37}, {192, 128, 2, 63, 51},
+    {192, 256, 2, 90, 0},
+};
+enum { Q8_WAYS = sizeof q8_ways / sizeof *q8_ways, Q8_SPLITS = 8, UNITS = 256, FEW_TOKENS = 16 };
+
+struct Q8Plan {
+    uint32_t way, splits, per;
+};
+
+// The way and number of column splits of the least estimated time. The estimate adds up the
+// steps of a unit's workgroups, as many at once as LDS holds, and for splits a second
+// launch with their sums written and read. Fitted to 144 sizes (1024 to 18432 rows, 1024
+// to 9216 columns, 17 to 2048 tokens): what it picks takes 5% longer than the best
+// of all ways and splits measured there on average, 26% at worst.
+static Q8Plan q8_plan(uint32_t rows, uint32_t cols, uint32_t tokens)
+{
+    const uint64_t steps = (cols + 127) / 128;
+    Q8Plan best = {0, 1, (uint32_t)steps};
+    uint64_t least = ~(uint64_t)0;
+    for (uint32_t w = 0; w < Q8_WAYS; w++) {
+        const Q8Way& way = q8_ways[w];
+        const uint64_t tiles = (uint64_t)((rows + way.rows - 1) / way.rows) *
+            ((tokens + way.tokens - 1) / way.tokens);
+        const uint64_t lds = way.buffers * (way.rows + way.tokens) * 128;
+        const uint64_t at_once = 160 * 1024 / lds < 4 ? 160 * 1024 / lds : 4;
+        for (uint32_t want = 1; want <= Q8_SPLITS && 2 * want <= steps + 1; want++) {
+            const uint64_t per = (steps + want - 1) / want, splits = (steps + per - 1) / per;
+            const uint64_t mine = (tiles * splits + UNITS - 1) / UNITS, rest = mine % at_once;
+            const auto step = [&](uint64_t n) {
+                return n * way.shared > way.alone ? n * way.shared : way.alone;
+            };
+            uint64_t time = per * (mine / at_once * step(at_once) + (rest ? step(rest) : 0));
+            if (splits > 1) {
+                // 2.6 us, and 8 bytes a sum at 5 TB/s, in 1 / 64 us.
+                time += 166 + splits * rows * tokens / 9766;
+            }
+            if (time < least) {
+                least = time;
+                best = {w, (uint32_t)splits, (uint32_t)per};
+            }
+        }
+    }
+    return best;
+}
+
+template <int MW, int NW, int WM, int WN, int B>
+static void q8_tiles(const Q8Args& a, hipStream_t s)
+{
+    const uint32_t m = (a.p.tiles + MW * WM - 1) / (MW * WM);
+    const uint32_t n = (a.tokens + 16 * NW * WN - 1) / (16 * NW * WN);
+    hipLaunchKernelGGL((k_q8_tiles<MW, NW, WM, WN, B>), dim3(m * n * a.splits), dim3(64 * WM * WN),
+        0, s, a, m, n);
+}
+
 extern "C" size_t lh_q8_scratch_bytes(uint32_t rows, uint32_t cols, uint32_t tokens)
 {
-    return 0;
+    if (tokens <= FEW_TOKENS) {
+        return 0;
+    }
+    const Q8Plan plan = q8_plan(rows, cols, tokens);
+    return plan.splits == 1 ? 0 : (size_t)plan.splits * tokens * ((rows + 15) / 16 * 64);
 }
 
 extern "C" int lh_launch_q8_matvec(const uint8_t* packed, const int8_t* x, size_t x_stride,
     const float* x_scales, float* y, size_t y_stride, uint32_t rows, uint32_t cols,
     uint32_t tokens, uint8_t* scratch, hipStream_t s)
 {
-    const Q8Args a = {packed, q8_shape(rows, cols), x, x_scales, y, x_stride, y_stride, tokens};
-    hipLaunchKernelGGL(k_q8_matvec, dim3(a.p.tiles, (tokens + 15) / 16), dim3(64), 0, s, a);
+    Q8Args a = {packed, q8_shape(rows, cols), x, x_scales, y, reinterpret_cast<int32_t*>(scratch),
+        x_stride, y_stride, tokens, 1, 0};
+    if (tokens <= FEW_TOKENS) {
+        if (tokens > 4 && a.p.tiles >= 384) {
+            hipLaunchKernelGGL(k_q8_few<2>, dim3((a.p.tiles + 1) / 2), dim3(64 * FEW_WAVES), 0, s, a);
+        } else {
+            hipLaunchKernelGGL(k_q8_few<1>, dim3(a.p.tiles), dim3(64 * FEW_WAVES), 0, s, a);
+        }
+        return (int)hipGetLastError();
+    }
+    const Q8Plan plan = q8_plan(rows, cols, tokens);
+    a.splits = plan.splits;
+    a.per = plan.per;
+    switch (plan.way) {
+    case 0: q8_tiles<1, 2, 4, 1, 4>(a, s); break;
+    case 1: q8_tiles<2, 2, 2, 2, 3>(a, s); break;
+    case 2: q8_tiles<4, 2, 2, 4, 2>(a, s); break;
+    case 3: q8_tiles<6, 4, 2, 2, 2>(a, s); break;
+    default: q8_tiles<6, 4, 2, 4, 2>(a, s); break;
+    }
+    const hipError_t e = hipGetLastError();
+    if (e || a.splits == 1) {
+        return (int)e;
+    }
+    hipLaunchKernelGGL(k_q8_join, dim3((rows + 1023) / 1024, tokens), dim3(256), 0, s, a);
     return (int)hipGetLastError();
 }
