@@ -2,94 +2,370 @@
 // lh_q8_norm).
 //
 // v = x, SiLU(x) * second, or gamma (h / sqrt(mean h^2 + 1e-5)) with h = x + second;
-// scale = max |v| / 127, code = rint(v / scale). A code that lies next to a border
-// between two would change with v's last bits, so v is formed in 64 bits, which is as
-// fast here as the bytes come.
-#include "lh_device.h"
+// scale = max |v| / 127, code = rint(v / scale). A code next to a border between two hangs
+// on v's last bits, so scales and codes are those of v in 64 bits. But 64 bits are
+// formed only where they decide: a quotient in FP32 is off by less than 2^-13, so
+// only one within 2^-12 of a border (one of 2000 to 4000) is formed again.
+// Bound: a row's bytes, read once into registers and written once. Measured: the norm with
+// the addition of 4096 rows of 3072 33.6 us, 4.9 TB/s (a large copy makes 4.7 to 5.2),
+// 4096 plain rows of 4096 16.2 us, 5.2 TB/s, SwiGLU of 2048 rows of 9216 45 us, 3.8 TB/s
+// (its exponential and two joins; with all of it in 64 bits 108); one row of the norm 4.1.
+// A row in memory twice, and in 64 bits throughout, took the norm 77 us.
 #include "lh_serving.h"
+#include "lh_topk.h"
 
 namespace lh {
 
-// Values c .. c + 3 of a row, and whether they are finite.
-struct Four {
-    double v[4];
-    bool finite;
-};
-
-template <int KIND>
-__device__ __forceinline__ float q8_input(const lh_q8_source& a, size_t row, uint32_t c)
+template <int J>
+__device__ __forceinline__ double xor_double(double v, uint32_t lane)
 {
-    const float x = a.x[row * a.x_stride + c];
-    return KIND == LH_Q8_NORM && a.second ? x + a.second[row * a.second_stride + c] : x;
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t)xor_word<J>((uint32_t)(u >> 32), lane) << 32 |
+        xor_word<J>((uint32_t)u, lane));
 }
 
-// The row's value at c; h of the norm.
-template <int KIND>
-__device__ __forceinline__ double q8_value(const lh_q8_source& a, size_t row, uint32_t c, float x)
+template <int J>
+__device__ __forceinline__ void join_lanes(double& sum, double& most, uint32_t lane)
 {
-    if (KIND == LH_Q8_SILU) {
-        return (double)x / (1.0 + exp(-(double)x)) *
-            (double)a.second[row * a.second_stride + c];
+    sum += xor_double<J>(sum, lane);
+    most = fmax(most, xor_double<J>(most, lane));
+    if constexpr (J > 1) {
+        join_lanes<J / 2>(sum, most, lane);
     }
-    return KIND == LH_Q8_NORM ? (double)a.gamma[c] * (double)x : (double)x;
 }
 
-// A workgroup a row.
-template <int KIND>
-__global__ void __launch_bounds__(256)
-k_q8_rows(lh_q8_source a)
+// Sum and maximum (of values that are not NaN) over a row's W waves, in every lane. Each
+// call of a workgroup has `shared` of its own.
+template <int W>
+__device__ __forceinline__ void join_row(double& sum, double& most, double (&shared)[2][W],
+    uint32_t lane, uint32_t wave)
 {
-    __shared__ double sums[4], mosts[4];
-    __shared__ uint32_t odd;
-    const size_t row = blockIdx.x;
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (threadIdx.x == 0) {
-        odd = 0;
-    }
-    __syncthreads();
-    double sum = 0, most = 0;
-    bool finite = true;
-    for (uint32_t c = threadIdx.x; c < a.width; c += 256) {
-        const float x = q8_input<KIND>(a, row, c);
-        if (KIND == LH_Q8_NORM) {
-            if (a.sum) {
-                a.sum[row * a.sum_stride + c] = x;
-            }
-            sum += (double)x * (double)x;
-        }
-        const double v = q8_value<KIND>(a, row, c, x);
-        finite &= __builtin_isfinite(v) && __builtin_isfinite(x);
-        most = fmax(most, fabs(v));
-    }
-    for (int s = 32; s; s >>= 1) {
-        sum += __shfl_xor(sum, s);
-        most = fmax(most, __shfl_xor(most, s));
+    join_lanes<32>(sum, most, lane);
+    if (W == 1) {
+        return;
     }
     if (lane == 0) {
-        sums[wave] = sum;
-        mosts[wave] = most;
-    }
-    if (!finite) {
-        odd = 1;
+        shared[0][wave] = sum;
+        shared[1][wave] = most;
     }
     __syncthreads();
-    sum = sums[0] + sums[1] + sums[2] + sums[3];
-    most = fmax(fmax(mosts[0], mosts[1]), fmax(mosts[2], mosts[3]));
-    const double r = KIND == LH_Q8_NORM ? 1.0 / sqrt(sum / a.width + 1e-5) : 1.0;
-    float scale = (float)(most * r / 127.0);
-    const bool bad = odd || !__builtin_isfinite(scale);
-    if (threadIdx.x == 0) {
-        a.scales[row] = bad ? __builtin_nanf("") : scale;
+    sum = shared[0][0];
+    most = shared[1][0];
+#pragma unroll
+    for (int i = 1; i < W; i++) {
+        sum += shared[0][i];
+        most = fmax(most, shared[1][i]);
     }
-    for (uint32_t c = threadIdx.x; c < a.width; c += 256) {
-        double v = 0;
-        if (!bad && scale > 0) {
-            const float x = KIND == LH_Q8_NORM && a.sum ? a.sum[row * a.sum_stride + c]
-                : q8_input<KIND>(a, row, c);
-            v = q8_value<KIND>(a, row, c, x) * r / (double)scale;
-            v = rint(fmin(fmax(v, -127.0), 127.0));
+}
+
+// SiLU(g) * u with an error below 2^-20 of itself, for g above -80 and results between
+// 2^-90 and 2^120.
+__device__ __forceinline__ float silu_near(float g, float u)
+{
+    const float e = exp_near(-fabsf(g)), part = __builtin_amdgcn_rcpf(1.0f + e);
+    return g * (g < 0 ? e * part : part) * u;
+}
+
+__device__ __forceinline__ double silu_wide(float g, float u)
+{
+    return (double)g / (1.0 + exp(-(double)g)) * (double)u;
+}
+
+// A row's value at column c in 64 bits, r the norm's factor.
+template <int KIND>
+__device__ __forceinline__ double q8_wide(const lh_q8_source& a, size_t row, uint32_t c, float h,
+    double r)
+{
+    if (KIND == LH_Q8_SILU) {
+        return silu_wide(a.x[row * a.x_stride + c], a.second[row * a.second_stride + c]);
+    }
+    return KIND == LH_Q8_NORM ? (double)a.gamma[c] * (double)h * r : (double)h;
+}
+
+__device__ __forceinline__ int q8_code_wide(double v, float scale)
+{
+    return (int)rint(fmin(fmax(v / (double)scale, -127.0), 127.0));
+}
+
+// Columns c .. c + 3 of a row; 0 past its end.
+__device__ __forceinline__ void load_quad(const float* row, uint32_t c, uint32_t width,
+    float (&v)[4])
+{
+    if (c + 3 < width) {
+        const float4 f = load4(row + c);
+        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        v[e] = c + e < width ? row[c + e] : 0.0f;
+    }
+}
+
+__device__ __forceinline__ void store_codes(int8_t* to, uint32_t c, uint32_t width,
+    const int (&code)[4])
+{
+    if (c + 3 < width) {
+        *reinterpret_cast<uint32_t*>(to + c) = (code[0] & 255) | (code[1] & 255) << 8 |
+            (code[2] & 255) << 16 | (uint32_t)code[3] << 24;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 3; e++) {
+        if (c + e < width) {
+            to[c + e] = (int8_t)code[e];
         }
-        a.codes[row * a.code_stride + c] = (int8_t)v;
+    }
+}
+
+// The row's h: x, or x + second.
+template <int KIND>
+__device__ __forceinline__ void load_h(const lh_q8_source& a, size_t row, uint32_t c,
+    float (&h)[4])
+{
+    load_quad(a.x + row * a.x_stride, c, a.width, h);
+    if (KIND == LH_Q8_NORM && a.second) {
+        float s[4];
+        load_quad(a.second + row * a.second_stride, c, a.width, s);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            h[e] += s[e];
+        }
+    }
+}
+
+__device__ __forceinline__ void store_h(const lh_q8_source& a, size_t row, uint32_t c,
+    const float (&h)[4])
+{
+    float* to = a.sum + row * a.sum_stride;
+    if (c + 3 < a.width) {
+        store4(to + c, make_float4(h[0], h[1], h[2], h[3]));
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 3; e++) {
+        if (c + e < a.width) {
+            to[c + e] = h[e];
+        }
+    }
+}
+
+// A row in W waves, Q quads of columns a lane, all in registers.
+template <int KIND, int W, int Q>
+__global__ void __launch_bounds__(W == 1 ? 256 : 64 * W)
+k_q8_rows(lh_q8_source a)
+{
+    constexpr uint32_t ROWS = W == 1 ? 4 : 1, STEP = 256 * W;
+    __shared__ double shared[KIND == LH_Q8_SILU ? 3 : 1][ROWS][2][W];
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t wave = all % W, mine = all / W;
+    const uint32_t first = 256 * wave + 4 * lane;
+    const size_t row = (size_t)blockIdx.x * ROWS + mine;
+    if (row >= a.tokens) {
+        return;   // of several rows in a workgroup, which meet at no barrier
+    }
+    float v[Q][4];
+    double sum = 0, most = 0;
+    bool bad = false;
+    float odd = 0;   // not 0: an Inf or NaN came in
+#pragma unroll
+    for (int q = 0; q < Q; q++) {
+        load_h<KIND>(a, row, first + q * STEP, v[q]);
+    }
+    float g[KIND == LH_Q8_NORM ? Q : 1][4], u[KIND == LH_Q8_SILU ? Q : 1][4];
+#pragma unroll
+    for (int q = 0; q < Q; q++) {
+        if (KIND == LH_Q8_NORM) {
+            load_quad(a.gamma, first + q * STEP, a.width, g[q]);
+        }
+        if (KIND == LH_Q8_SILU) {
+            load_quad(a.second + row * a.second_stride, first + q * STEP, a.width, u[q]);
+        }
+    }
+    float near = 0;
+#pragma unroll
+    for (int q = 0; q < Q; q++) {
+        const uint32_t c = first + q * STEP;
+        if (KIND == LH_Q8_NORM && a.sum && c < a.width) {
+            store_h(a, row, c, v[q]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (KIND == LH_Q8_NORM) {
+                const double h = v[q][e], w = (double)g[q][e] * h;
+                sum += h * h;
+                most = fmax(most, fabs(w));
+                bad |= !(fabs(w) <= 1e300);
+            } else if (KIND == LH_Q8_SILU) {
+                odd += v[q][e] * 0.0f + u[q][e] * 0.0f;
+                bad |= v[q][e] < -80.0f;   // 64 bits for the row
+                v[q][e] = silu_near(v[q][e], u[q][e]);
+                near = fmaxf(near, fabsf(v[q][e]));
+            } else {
+                odd += v[q][e] * 0.0f;
+                near = fmaxf(near, fabsf(v[q][e]));
+            }
+        }
+    }
+    const double inf = __builtin_inf();
+    double r = 1;
+    bool wide = false;   // the whole row in 64 bits
+    if (KIND == LH_Q8_NORM) {
+        most = bad ? inf : most;
+        join_row<W>(sum, most, shared[0][mine], lane, wave);
+        wide = !(most >= 0x1p-90 && most < 0x1p120);
+        r = 1.0 / sqrt(sum / a.width + 1e-5);
+        most = sum < inf ? most * r : inf;   // a NaN too
+    } else if (KIND == LH_Q8_ROWS) {
+        most = odd == 0 ? (double)near : inf;
+        join_row<W>(sum, most, shared[0][mine], lane, wave);
+    } else {
+        // First the largest in FP32 (-80 and below, Inf and NaN as larger ones still), then
+        // those near it in 64 bits.
+        sum = odd == 0 ? 0 : 1;
+        most = bad || !(near < 0x1p120f) ? 0x1p121 : (double)near;
+        join_row<W>(sum, most, shared[0][mine], lane, wave);
+        const bool none = sum != 0;
+        wide = !(most >= 0x1p-90 && most < 0x1p120);
+        const float from = (float)most * (1 - 0x1p-18f);
+        most = 0;
+        if (!none) {
+#pragma unroll
+            for (int q = 0; q < Q; q++) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t c = first + q * STEP + e;
+                    if (c < a.width && (wide || fabsf(v[q][e]) >= from)) {
+                        most = fmax(most, fabs(q8_wide<KIND>(a, row, c, 0, 1)));
+                    }
+                }
+            }
+        }
+        join_row<W>(sum, most, shared[1][mine], lane, wave);
+        most = none ? inf : most;
+    }
+    const float scale = (float)(most / 127.0);
+    const bool fine = scale < __builtin_inff();
+    if (lane == 0 && wave == 0) {
+        a.scales[row] = fine ? scale : __builtin_nanf("");
+    }
+    // v times this is the quotient, off by a few parts of 2^23; where that leaves FP32's
+    // range all of the row takes 64 bits.
+    const float by = fine && scale > 0 ? (float)(r / (double)scale) : 0.0f;
+    wide |= !(by >= 0x1p-100f && by <= 0x1p100f) || !(scale >= 0x1p-100f);
+    int8_t* codes = a.codes + row * a.code_stride;
+#pragma unroll
+    for (int q = 0; q < Q; q++) {
+        const uint32_t c = first + q * STEP;
+        if (c >= a.width) {
+            continue;
+        }
+        int code[4] = {0, 0, 0, 0};
+        if (fine && scale > 0) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float w = KIND == LH_Q8_NORM ? g[q][e] * v[q][e] : v[q][e];
+                const float t = w * by, n = rintf(t);
+                code[e] = (int)n;
+                const bool border = fabsf(fabsf(t - n) - 0.5f) < 0x1p-12f;
+                if ((wide || border) && c + e < a.width) {
+                    code[e] = q8_code_wide(q8_wide<KIND>(a, row, c + e, v[q][e], r), scale);
+                }
+                code[e] = code[e] < -127 ? -127 : code[e] > 127 ? 127 : code[e];
+            }
+        }
+        store_codes(codes, c, a.width, code);
+    }
+}
+
+// Rows that registers do not hold, column by column in 64 bits, twice.
+template <int KIND>
+__global__ void __launch_bounds__(1024)
+k_q8_wide_rows(lh_q8_source a)
+{
+    __shared__ double shared[2][16];
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const size_t row = blockIdx.x;
+    double sum = 0, most = 0;
+    for (uint32_t c = threadIdx.x; c < a.width; c += 1024) {
+        float h = a.x[row * a.x_stride + c];
+        float odd = h;
+        if (KIND == LH_Q8_NORM) {
+            h = a.second ? h + a.second[row * a.second_stride + c] : h;
+            odd = h;
+            if (a.sum) {
+                a.sum[row * a.sum_stride + c] = h;
+            }
+            sum += (double)h * (double)h;
+        } else if (KIND == LH_Q8_SILU) {
+            odd = odd * 0.0f + a.second[row * a.second_stride + c] * 0.0f;
+        }
+        const double v = fabs(q8_wide<KIND>(a, row, c, h, 1));
+        most = fmax(most, __builtin_isfinite(odd) && v <= 1e300 ? v : __builtin_inf());
+    }
+    join_row<16>(sum, most, shared, lane, wave);
+    const double r = KIND == LH_Q8_NORM ? 1.0 / sqrt(sum / a.width + 1e-5) : 1.0;
+    const float scale = (float)(most * r / 127.0);
+    const bool fine = scale < __builtin_inff();
+    if (threadIdx.x == 0) {
+        a.scales[row] = fine ? scale : __builtin_nanf("");
+    }
+    // The same thread's columns as before: a sum in place is its own.
+    for (uint32_t c = threadIdx.x; c < a.width; c += 1024) {
+        int code = 0;
+        if (fine && scale > 0) {
+            float h = 0;
+            if (KIND == LH_Q8_NORM && a.sum) {
+                h = a.sum[row * a.sum_stride + c];
+            } else if (KIND != LH_Q8_SILU) {
+                h = a.x[row * a.x_stride + c];
+                h = KIND == LH_Q8_NORM && a.second ? h + a.second[row * a.second_stride + c] : h;
+            }
+            code = q8_code_wide(q8_wide<KIND>(a, row, c, h, r), scale);
+        }
+        a.codes[row * a.code_stride + c] = (int8_t)code;
+    }
+}
+
+template <int KIND, int W, int Q>
+static void q8_rows(const lh_q8_source& a, hipStream_t s)
+{
+    constexpr uint32_t rows = W == 1 ? 4 : 1;
+    hipLaunchKernelGGL((k_q8_rows<KIND, W, Q>), dim3((a.tokens + rows - 1) / rows),
+        dim3(64 * W * rows), 0, s, a);
+}
+
+// Few waves with up to four quads a lane: 3072 columns x 4096 tokens of the norm take four
+// waves 33.4 us, twelve 34.8 (SwiGLU 25.8 and 39.6), 9216 x 2048 sixteen 58.1. Waves
+// that the four SIMDs do not share evenly take longer: three 37.1, nine 74.9.
+template <int KIND>
+static void q8_rows(const lh_q8_source& a, hipStream_t s)
+{
+    const uint32_t quads = (a.width + 255) / 256;   // of a lane in one wave
+    switch (quads) {
+    case 1: q8_rows<KIND, 1, 1>(a, s); return;
+    case 2: q8_rows<KIND, 1, 2>(a, s); return;
+    case 3: q8_rows<KIND, 1, 3>(a, s); return;
+    case 4: q8_rows<KIND, 1, 4>(a, s); return;
+    }
+    if (quads <= 8) {
+        q8_rows<KIND, 4, 2>(a, s);
+    } else if (quads <= 12) {
+        q8_rows<KIND, 4, 3>(a, s);
+    } else if (quads <= 16) {
+        q8_rows<KIND, 4, 4>(a, s);
+    } else if (quads <= 24) {
+        q8_rows<KIND, 8, 3>(a, s);
+    } else if (quads <= 32) {
+        q8_rows<KIND, 8, 4>(a, s);
+    } else if (quads <= 48) {
+        q8_rows<KIND, 16, 3>(a, s);
+    } else if (quads <= 64) {
+        q8_rows<KIND, 16, 4>(a, s);
+    } else {
+        hipLaunchKernelGGL(k_q8_wide_rows<KIND>, dim3(a.tokens), dim3(1024), 0, s, a);
     }
 }
 
@@ -99,13 +375,12 @@ using namespace lh;
 
 extern "C" int lh_launch_q8_rows(int kind, const lh_q8_source* rows, hipStream_t s)
 {
-    const dim3 grid(rows->tokens), block(256);
     if (kind == LH_Q8_SILU) {
-        hipLaunchKernelGGL(k_q8_rows<LH_Q8_SILU>, grid, block, 0, s, *rows);
+        q8_rows<LH_Q8_SILU>(*rows, s);
     } else if (kind == LH_Q8_NORM) {
-        hipLaunchKernelGGL(k_q8_rows<LH_Q8_NORM>, grid, block, 0, s, *rows);
+        q8_rows<LH_Q8_NORM>(*rows, s);
     } else {
-        hipLaunchKernelGGL(k_q8_rows<LH_Q8_ROWS>, grid, block, 0, s, *rows);
+        q8_rows<LH_Q8_ROWS>(*rows, s);
     }
     return (int)hipGetLastError();
 }

@@ -97,6 +97,22 @@ def test_rows(gpu, tokens, width):
         assert np.array_equal(again[0], got[0]) and np.array_equal(again[1], got[1])
 
 
+@pytest.mark.parametrize("width", [w + d for w in (256, 512, 768, 1024, 2048, 3072, 4096, 6144, 8192,
+                                                  12288, 16384) for d in (-1, 0, 1)])
+def test_row_widths(gpu, width):
+    """To either side of each way to hold a row, a number of rows that fills no workgroup."""
+    rng = np.random.default_rng(width)
+    x = (rng.normal(size=(6, width)) * np.exp(rng.normal(size=width))).astype(np.float32)
+    y = rng.normal(size=(6, width)).astype(np.float32)
+    gamma = (1 + 0.3 * rng.normal(size=width)).astype(np.float32)
+    q8.check_rows(*run_rows(gpu, x), x.astype(np.float64))
+    q8.check_rows(*run_silu(gpu, x, y), q8.silu(x, y))
+    h, v = q8.norm(x, y, gamma)
+    got = run_norm(gpu, x, y, gamma, kept="x", pad=1)
+    assert np.array_equal(got[0], h)
+    q8.check_rows(got[1], got[2], v)
+
+
 def test_rows_ties_and_ranges(gpu):
     """Halves go to even codes, whatever the scale; constant, zero, subnormal, largest
     and nonfinite rows."""
