@@ -127,7 +127,7 @@ struct BeamShared {
     double base[LH_BEAMS], log_z[LH_BEAMS];
     float most[LH_BEAMS];
     uint32_t kind[LH_BEAMS], bad, count;
-    Place lists[WAVES][64];
+    Place bound, lists[WAVES][64];
     Place places[PLACES];
 };
 enum { BEAM_NONE, BEAM_LIVE, BEAM_DONE };
@@ -171,8 +171,7 @@ __device__ __forceinline__ Place join_places(Place (&lists)[WAVES][64], Place p,
     return p;
 }
 
-// grid (groups). Each list is falling, so the keep-th best of the lists' first places
-// bounds the group's best from below, and only `keep` lists reach it.
+// grid (groups).
 __global__ void __launch_bounds__(64 * WAVES)
 k_beam_join(BeamArgs a)
 {
@@ -185,6 +184,7 @@ k_beam_join(BeamArgs a)
         sh.bad = 0;
         sh.count = 0;
     }
+    const uint32_t lists = c.beams * a.parts;
     __syncthreads();
     for (uint32_t b = wave; b < c.beams; b += WAVES) {
         const float s = c.scores[row + b];
@@ -194,7 +194,7 @@ k_beam_join(BeamArgs a)
             r = a.ranges[(row + b) * a.parts + lane];
         }
         rescale(r, wave_max64(r.m));
-        r.z = wave_sum(r.z);
+        r.z = wave_sum(r.z, lane);
         const bool odd = __ballot(r.bad != 0) != 0 || !(s < __builtin_inff());
         if (lane == 0) {
             sh.kind[b] = s == -__builtin_inff() ? BEAM_NONE : live ? BEAM_LIVE : BEAM_DONE;
@@ -219,34 +219,43 @@ k_beam_join(BeamArgs a)
         }
         return;
     }
-    // A list a lane of the first four waves.
-    const uint32_t lists = c.beams * a.parts;
     Place p = {0, 0};
-    if (threadIdx.x < lists) {
-        p = candidate(a, sh, row, threadIdx.x / a.parts, threadIdx.x % a.parts, 0);
-    }
-    p = sort_places(p, lane, true);
-    p = join_places(sh.lists, p, (lists + 63) / 64, wave, lane);
-    if (threadIdx.x == c.keep - 1) {
-        sh.places[0] = p;
-    }
-    __syncthreads();
-    const Place bound = sh.places[0];
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < lists * c.keep; i += 64 * WAVES) {
-        const uint32_t list = i / c.keep;
-        const Place mine = candidate(a, sh, row, list / a.parts, list % a.parts, i % c.keep);
-        if (mine.score && !(bound > mine)) {
-            sh.places[atomicAdd(&sh.count, 1u)] = mine;
+    uint32_t n = lists * c.keep;
+    if (n <= 64 * WAVES) {
+        // A candidate a thread.
+        const uint32_t list = threadIdx.x / c.keep;
+        if (threadIdx.x < n) {
+            p = candidate(a, sh, row, list / a.parts, list % a.parts, threadIdx.x % c.keep);
         }
-    }
-    __syncthreads();
-    const uint32_t n = sh.count;
-    p = {0, 0};
-    for (uint32_t i = 64 * wave; i < n; i += 64 * WAVES) {
-        const Place mine = i + lane < n ? sh.places[i + lane] : Place{0, 0};
-        p = i < 64 * WAVES ? sort_places(mine, lane, true)
-            : merge_places(p, sort_places(mine, lane, false), lane);
+        p = sort_places(p, lane, true);
+    } else {
+        // Lists are falling, so the keep-th best of their first places bounds the group's best
+        // from below, and only `keep` lists reach it. A list a lane of the first four waves.
+        if (threadIdx.x < lists) {
+            p = candidate(a, sh, row, threadIdx.x / a.parts, threadIdx.x % a.parts, 0);
+        }
+        p = sort_places(p, lane, true);
+        p = join_places(sh.lists, p, (lists + 63) / 64, wave, lane);
+        if (threadIdx.x == c.keep - 1) {
+            sh.bound = p;
+        }
+        __syncthreads();
+        const Place bound = sh.bound;
+        for (uint32_t i = threadIdx.x; i < n; i += 64 * WAVES) {
+            const uint32_t list = i / c.keep;
+            const Place mine = candidate(a, sh, row, list / a.parts, list % a.parts, i % c.keep);
+            if (mine.score && !(bound > mine)) {
+                sh.places[atomicAdd(&sh.count, 1u)] = mine;
+            }
+        }
+        __syncthreads();
+        n = sh.count;
+        p = {0, 0};
+        for (uint32_t i = 64 * wave; i < n; i += 64 * WAVES) {
+            const Place mine = i + lane < n ? sh.places[i + lane] : Place{0, 0};
+            p = i < 64 * WAVES ? sort_places(mine, lane, true)
+                : merge_places(p, sort_places(mine, lane, false), lane);
+        }
     }
     p = join_places(sh.lists, p, (n + 63) / 64 < WAVES ? (n + 63) / 64 : WAVES, wave, lane);
     if (threadIdx.x < c.keep) {
@@ -316,9 +325,12 @@ __device__ __forceinline__ uint32_t open_column(const ReorderArgs& a, int32_t le
     return length < 0 ? 0 : (uint32_t)length / a.page_size;
 }
 
-// grid (pieces, sequences, layers): the open pages that are copied. No page is both
-// read and written: the pages read stay their first child's, those written belong to
-// beams without children.
+// grid (pieces, sequences, layers and, for other tables than the old, one): the open pages
+// that are copied, then the sequences' rows. No page is both read and written: the pages
+// read stay their first child's, those written belong to beams without children.
+// Bound: the pages' bytes; 8 groups of 8 beams in FP16 pages of 26 layers (436 MB
+// both ways) 67 us, 6.5 TB/s; 4 beams in 4-bit pages 4.3 us, the loads of parents, length,
+// page ids and page one after another.
 __global__ void __launch_bounds__(256)
 k_beam_copy(ReorderArgs a)
 {
@@ -328,12 +340,21 @@ k_beam_copy(ReorderArgs a)
     const int32_t length = a.length[row];
     const Family f(a.parent + row, a.beams, lane);
     const int32_t parent = __builtin_amdgcn_readlane(f.parent, beam);
+    const uint32_t owner = __builtin_amdgcn_readlane(f.owner(lane), beam);
     const uint32_t column = open_column(a, length);
+    if (blockIdx.z == a.layers) {
+        const int32_t* full = a.table + (row + (parent < 0 ? owner : parent)) * a.width;
+        const int32_t* own = a.table + (row + owner) * a.width;
+        int32_t* out = a.table_out + (row + beam) * a.width;
+        for (uint32_t c = blockIdx.x * 256 + threadIdx.x; c < a.width; c += gridDim.x * 256) {
+            out[c] = (c < column ? full : own)[c];
+        }
+        return;
+    }
     if (parent < 0 || f.keeps >> beam & 1 || length <= 0 || length % a.page_size == 0 ||
         column >= a.width) {
         return;
     }
-    const uint32_t owner = __builtin_amdgcn_readlane(f.owner(lane), beam);
     const int32_t from = a.table[(row + parent) * a.width + column];
     const int32_t to = a.table[(row + owner) * a.width + column];
     if (from < 0 || to < 0 || (uint32_t)from >= a.page_count || (uint32_t)to >= a.page_count) {
@@ -348,8 +369,8 @@ k_beam_copy(ReorderArgs a)
     }
 }
 
-// grid (column tiles, groups): all rows of a group are read before one is written, so
-// the tables may be the same.
+// grid (column tiles, groups): rows of tables in place. All of a group are read before one
+// is written.
 __global__ void __launch_bounds__(256)
 k_beam_tables(ReorderArgs a)
 {
@@ -429,8 +450,10 @@ extern "C" int lh_launch_beam_reorder(const lh_paged_cache* caches, uint32_t lay
     a.layers = layers, a.beams = beams, a.width = width;
     a.page_size = caches->page_size, a.page_count = caches->pages;
     const uint32_t pieces = (uint32_t)((a.page_bytes + 16383) / 16384);
-    hipLaunchKernelGGL(k_beam_copy, dim3(pieces, groups * beams, layers), dim3(256), 0, s, a);
-    if (const hipError_t e = hipGetLastError()) {
+    hipLaunchKernelGGL(k_beam_copy, dim3(pieces, groups * beams, layers + (table != table_out)),
+        dim3(256), 0, s, a);
+    const hipError_t e = hipGetLastError();
+    if (e || table != table_out) {
         return (int)e;
     }
     const uint32_t tiles = (width + 63) / 64;

@@ -107,12 +107,22 @@ __device__ __forceinline__ uint32_t sort_ranks(uint32_t rank, uint32_t lane)
     return half_merge<32>(rank, lane, false);
 }
 
-__device__ __forceinline__ double wave_sum(double v)
+template <int J>
+__device__ __forceinline__ double xor_double(double v, uint32_t lane)
 {
-    for (int s = 32; s; s >>= 1) {
-        v += __shfl_xor(v, s);
-    }
-    return v;
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t)xor_word<J>((uint32_t)(u >> 32), lane) << 32 |
+        xor_word<J>((uint32_t)u, lane));
+}
+
+__device__ __forceinline__ double wave_sum(double v, uint32_t lane)
+{
+    v += xor_double<32>(v, lane);
+    v += xor_double<16>(v, lane);
+    v += xor_double<8>(v, lane);
+    v += xor_double<4>(v, lane);
+    v += xor_double<2>(v, lane);
+    return v + xor_double<1>(v, lane);
 }
 
 // A range of a row: its maximum, the sums relative to it, whether it holds a NaN or
@@ -321,9 +331,9 @@ __device__ __forceinline__ void scan_part(PartShared& sh, const float* x, uint32
         }
     }
     r.bad = __ballot(bad) != 0;
-    r.z = wave_sum(r.z);
+    r.z = wave_sum(r.z, lane);
     if (WEIGHTED) {
-        r.w = wave_sum(r.w);
+        r.w = wave_sum(r.w, lane);
     }
     if (lane == 0) {
         sh.ranges[wave] = r;
@@ -359,8 +369,8 @@ __device__ __forceinline__ void scan_part(PartShared& sh, const float* x, uint32
         r.z *= (double)f;
     }
     r.m = to;
-    r.z = wave_sum(r.z);
-    r.w = wave_sum(r.w);
+    r.z = wave_sum(r.z, lane);
+    r.w = wave_sum(r.w, lane);
     r.bad = __ballot(r.bad != 0) != 0;
 }
 

@@ -122,8 +122,8 @@ k_logprob_join(LogprobArgs a)
         return;
     }
     rescale(r, wave_max64(r.m));
-    r.z = wave_sum(r.z);
-    r.w = wave_sum(r.w);
+    r.z = wave_sum(r.z, lane);
+    r.w = wave_sum(r.w, lane);
     r.bad = __ballot(r.bad != 0) != 0;
     finish(a, row, r, key, lane);
 }

@@ -17,14 +17,6 @@
 namespace lh {
 
 template <int J>
-__device__ __forceinline__ double xor_double(double v, uint32_t lane)
-{
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    return __builtin_bit_cast(double, (uint64_t)xor_word<J>((uint32_t)(u >> 32), lane) << 32 |
-        xor_word<J>((uint32_t)u, lane));
-}
-
-template <int J>
 __device__ __forceinline__ void join_lanes(double& sum, double& most, uint32_t lane)
 {
     sum += xor_double<J>(sum, lane);
