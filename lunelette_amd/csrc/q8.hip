@@ -3,8 +3,8 @@
 // Packed weights: tiles of 16 rows x 64 columns, row tile by row tile, the codes of
 // all tiles first. A tile's 1 KiB holds for lane l = 16 g + r of a wave row r's columns
 // 16 g .. 16 g + 15: the operand of a 16x16x64 matrix instruction. Then the FP32 scales
-// of the rows. Rows and columns past the matrix have codes and scales of 0, so what
-// the activations hold past their last column adds nothing.
+// of the rows. Rows and columns past the matrix, to a multiple of 16 and of 128, have
+// codes and scales of 0, so what the activations hold past their last column adds nothing.
 #include "lh_mfma.h"
 #include "lh_serving.h"
 
@@ -18,7 +18,7 @@ struct Q8Shape {
 
 static Q8Shape q8_shape(uint32_t rows, uint32_t cols)
 {
-    return {rows, cols, (rows + 15) / 16, (cols + 63) / 64};
+    return {rows, cols, (rows + 15) / 16, (cols + 127) / 128 * 2};
 }
 
 __device__ __forceinline__ const float* q8_scales(const uint8_t* packed, const Q8Shape& p)
@@ -220,14 +220,18 @@ __device__ __forceinline__ void q8_meet()
 // tiles of rows and NT = WN * NW tiles of tokens, a wave MW x NW of them, over a split
 // of the columns. 128 columns (a step) of both operands at a time go to LDS as they are
 // multiplied, in B buffers: one is multiplied while the others fill.
-// Bound: at large tiles the way of the operands from L2 to LDS beside the matrix
-// instructions: 18432 x 3072 for 2048 tokens takes 117 to 120 us, 1.95e15 operations a
-// second (without the matrix instructions 100). Measured there, too:
-// tiles of 256 x 256 136 us (576 items leave a quarter of the chip idle in their
-// third turn; 8192^3, which they fill, 2.37e15 a second), 128 x 256 in three buffers 147,
-// workgroups that go on to their next item 138 (registers), activations in pieces of 64
-// columns of 16 tokens 134 (half a cache line of each row a request), other starting
-// columns for each workgroup 119 to 124.
+// Bound: at large tiles matrix instructions and the operands' way from L2 to LDS, which the
+// one barrier a step lets overlap in part. 18432 x 3072 for 2048 tokens takes 118 us, 1.97e15
+// operations a second, with cold inputs and outputs 130 (256 x 256 tiles: without the
+// matrix instructions 100, without loads and reads 110, without stores 10 less, cold 20
+// less; the matrix instructions alone reach 3.5e15 to 4.1e15 on random codes).
+// Measured there, too: tiles of 192 x 256 in one workgroup a unit 115, cold 131, but 82
+// against 77 for 1024 tokens and 94 against 78 for 3072 x 9216; 256 x 256 125, cold 139
+// (8192^3, which they fill: 2.37e15 a second); 128 x 256 in three buffers 144; workgroups
+// that go on to their next item 138 (registers); four waves of 96 x 128 172 (registers);
+// activations in pieces of 64 columns of 16 tokens 134 (half a cache line of each row a
+// request); other starting columns for each workgroup, stores past the caches, priorities
+// of waves or of workgroups: no gain.
 template <int MW, int NW, int WM, int WN, int B>
 __global__ void __launch_bounds__(64 * WM * WN, 2)
 k_q8_tiles(Q8Args a, uint32_t mtiles, uint32_t ntiles)
@@ -249,7 +253,7 @@ k_q8_tiles(Q8Args a, uint32_t mtiles, uint32_t ntiles)
         : (blockIdx.x & 7) * (gridDim.x / 8) + (blockIdx.x >> 3);
     const uint32_t split = id % a.splits;
     id /= a.splits;
-    const uint32_t group = ntiles >= 8 ? 4 : 32 / ntiles;
+    const uint32_t group = ntiles >= 8 ? 8 : 32 / ntiles;
     const uint32_t base = id / (group * ntiles) * group, in = id % (group * ntiles);
     const uint32_t rows = mtiles - base < group ? mtiles - base : group;
     const uint32_t tile0 = (base + in % rows) * MT, token0 = in / rows * (NT * 16);
@@ -280,10 +284,10 @@ k_q8_tiles(Q8Args a, uint32_t mtiles, uint32_t ntiles)
         step = step < end ? step : end - 1;
 #pragma unroll
         for (int n = 0; n < AP; n++) {
-            const uint32_t f = AP * wave + n, b = 2 * step + (f & 1);
+            const uint32_t f = AP * wave + n;
             __builtin_amdgcn_global_load_lds(
                 (const __attribute__((address_space(1))) void*)(wfrom[n] +
-                    (size_t)(b < a.p.blocks ? b : a.p.blocks - 1) * 1024),
+                    (size_t)(2 * step + (f & 1)) * 1024),
                 (__attribute__((address_space(3))) void*)(to + f * 1024), 16, 0, 0);
         }
         const uint32_t col = 128 * step + word;
@@ -322,7 +326,6 @@ k_q8_tiles(Q8Args a, uint32_t mtiles, uint32_t ntiles)
     };
     auto multiply = [&](const i32x4 (&w)[MW], const i32x4 (&x)[NW])
         __attribute__((always_inline)) {
-        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int m = 0; m < MW; m++) {
 #pragma unroll
@@ -330,22 +333,35 @@ k_q8_tiles(Q8Args a, uint32_t mtiles, uint32_t ntiles)
                 acc[m][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[m], x[n], acc[m][n], 0, 0, 0);
             }
         }
-        __builtin_amdgcn_s_setprio(0);
     };
     // vmcnt(B - 2 steps' pieces), lgkmcnt(0): the next step's pieces, this wave's reads.
     constexpr int LEFT = (B - 2) * (AP + BP);
     constexpr int WAIT = 0x0070 | (LEFT & 15) | (LEFT >> 4) << 14;
     i32x4 w0[MW], x0[NW], w1[MW], x1[NW];
+    // The order that the compiler is held to: reads and loads among the matrix instructions,
+    // which take 16 cycles each, not all ahead of them (2048 tokens below: 4 us less).
+    constexpr int MFMA = 8, LOAD = 16, READ = 256, BETWEEN = MW * NW / (MW + NW);
     // Step s in `now`, whose first half is in registers; the next B - 2 are on their way.
     auto turn = [&](uint32_t s, uint8_t* now, uint8_t* then) __attribute__((always_inline)) {
         read(now, 1, w1, x1);
         multiply(w0, x0);
+#pragma unroll
+        for (int i = 0; i < MW + NW; i++) {
+            __builtin_amdgcn_sched_group_barrier(READ, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(MFMA, BETWEEN, 0);
+        }
         __builtin_amdgcn_sched_barrier(0);
         q8_meet<WAIT>();
         fetch(s + B, now);
         read(then, 0, w0, x0);
-        if (2 * s + 1 < a.p.blocks) {
-            multiply(w1, x1);
+        multiply(w1, x1);
+#pragma unroll
+        for (int i = 0; i < MW + NW; i++) {
+            if (i < AP + BP) {
+                __builtin_amdgcn_sched_group_barrier(LOAD, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(READ, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(MFMA, BETWEEN, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
         return s + 1 < end;
@@ -453,8 +469,8 @@ struct Q8Way {
     uint32_t rows, tokens, buffers, alone, shared;
 };
 static const Q8Way q8_ways[] = {
-    {64, 32, 4, 14, 11}, {64, 64, 3, 20, 16}, {128, 128, 2, 44, 37}, {192, 128, 2, 63, 51},
-    {192, 256, 2, 90, 0},
+    {64, 32, 4, 13, 11}, {64, 64, 3, 18, 15}, {64, 128, 3, 24, 24}, {128, 128, 2, 46, 37},
+    {192, 128, 2, 64, 50},
 };
 enum { Q8_WAYS = sizeof q8_ways / sizeof *q8_ways, Q8_SPLITS = 8, UNITS = 256, FEW_TOKENS = 16 };
 
@@ -464,9 +480,10 @@ struct Q8Plan {
 
 // The way and number of column splits of the least estimated time. The estimate adds up the
 // steps of a unit's workgroups, as many at once as LDS holds, and for splits a second
-// launch with their sums written and read. Fitted to 144 sizes (1024 to 18432 rows, 1024
-// to 9216 columns, 17 to 2048 tokens): what it picks takes 5% longer than the best
-// of all ways and splits measured there on average, 26% at worst.
+// launch with their sums written and read. Fitted to 180 sizes (1024 to 18432 rows, 1024
+// to 9216 columns, 17 to 2048 tokens, cold weights): what it picks takes 4% longer on
+// average, 31% at worst, than the best measured there of all splits of ten tiles (these
+// and 32 x 64, 64 x 64 and 64 x 128 and 128 x 128 in other waves, 192 x 256).
 static Q8Plan q8_plan(uint32_t rows, uint32_t cols, uint32_t tokens)
 {
     const uint64_t steps = (cols + 127) / 128;
@@ -486,8 +503,8 @@ static Q8Plan q8_plan(uint32_t rows, uint32_t cols, uint32_t tokens)
             };
             uint64_t time = per * (mine / at_once * step(at_once) + (rest ? step(rest) : 0));
             if (splits > 1) {
-                // 2.6 us, and 8 bytes a sum at 5 TB/s, in 1 / 64 us.
-                time += 166 + splits * rows * tokens / 9766;
+                // 2.9 us, and 8 bytes a sum at 4.9 TB/s, in 1 / 64 us.
+                time += 185 + splits * rows * tokens / 9475;
             }
             if (time < least) {
                 least = time;
@@ -536,9 +553,9 @@ extern "C" int lh_launch_q8_matvec(const uint8_t* packed, const int8_t* x, size_
     switch (plan.way) {
     case 0: q8_tiles<1, 2, 4, 1, 4>(a, s); break;
     case 1: q8_tiles<2, 2, 2, 2, 3>(a, s); break;
-    case 2: q8_tiles<4, 2, 2, 4, 2>(a, s); break;
-    case 3: q8_tiles<6, 4, 2, 2, 2>(a, s); break;
-    default: q8_tiles<6, 4, 2, 4, 2>(a, s); break;
+    case 2: q8_tiles<2, 2, 2, 4, 3>(a, s); break;
+    case 3: q8_tiles<4, 2, 2, 4, 2>(a, s); break;
+    default: q8_tiles<6, 4, 2, 2, 2>(a, s); break;
     }
     const hipError_t e = hipGetLastError();
     if (e || a.splits == 1) {

@@ -211,7 +211,7 @@ static int q8_sizes(size_t rows, size_t cols)
 
 size_t lh_q8_bytes(size_t rows, size_t cols)
 {
-    return q8_sizes(rows, cols) ? (rows + 15) / 16 * ((cols + 63) / 64 * 1024 + 64) : 0;
+    return q8_sizes(rows, cols) ? (rows + 15) / 16 * ((cols + 127) / 128 * 2048 + 64) : 0;
 }
 
 int lh_q8_pack(const int8_t *d_codes, const float *d_scales, size_t rows, size_t cols,
