@@ -122,42 +122,52 @@ __device__ __forceinline__ float4 q8_row_scales(const Q8Args& a, uint32_t row)
     return *reinterpret_cast<const float4*>(q8_scales(a.packed, a.p) + row);
 }
 
-// The product of up to 16 tokens. A workgroup takes RT tiles of rows, its eight waves a slice
-// of the columns each; a wave asks for U blocks of its slice at once and for another
-// whenever it has multiplied one. The sums meet in LDS.
+// The product of NT tiles of 16 tokens, one or two. A workgroup takes RT tiles of rows, its
+// eight waves a slice of the columns each; a wave asks for U blocks of its slice at once
+// and for another whenever it has multiplied one. The sums meet in LDS.
 // Bound: the weights' bytes. Measured, cold weights: 18432 x 3072 (57 MB) for one token
-// 10.5 us, 5.4 TB/s, 131072 x 3072 for eight 59 us, 6.8 TB/s; 3072 x 9216 6.8 us, of
-// which a launch and the first bytes' way are 4. Two tiles of rows share the tokens'
-// words where these are 16 rows apart each and there are workgroups enough: 18432 x 3072
-// for 16 tokens 14.0 us (one tile 14.7), 6144 x 3072 for eight 5.7 (6.2); but for one
-// token 11.8 (10.5). More loads on their way (nine blocks) or fewer (three): no gain.
-enum { FEW_WAVES = 8, FEW_BLOCKS = 6 };
+// 10.4 us, 5.4 TB/s, 131072 x 3072 for eight 59 us, 6.8 TB/s; 3072 x 9216 6.7 us, of
+// which a launch and the first bytes' way are 4. More tokens' words are 16 rows apart each,
+// which a request takes half a cache line of: 3072 x 9216 for 16 tokens 10.2 us. Two tiles
+// of rows share them where there are workgroups enough: 18432 x 3072 for 16 tokens 14.0
+// us (one tile 14.7), 6144 x 3072 for eight 5.7 (6.2), for 24 7.4 (9.2); but for one token
+// 11.8 (10.4), and 3072 x 9216 for 16 12.7. Nine blocks on their way or three, sixteen
+// waves or four: no gain.
+enum { FEW_WAVES = 8 };
 
-template <int RT>
+template <int RT, int NT>
 __global__ void __launch_bounds__(64 * FEW_WAVES)
 k_q8_few(Q8Args a)
 {
-    constexpr int W = FEW_WAVES, U = FEW_BLOCKS;
-    __shared__ i32x4 sums[W][RT][64];
+    constexpr int W = FEW_WAVES, U = RT * NT == 4 ? 3 : 6;
+    __shared__ i32x4 sums[W][RT * NT][64];
     const uint32_t lane = threadIdx.x & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t tile = blockIdx.x * RT, token = lane & 15;
+    const uint32_t tile = blockIdx.x * RT;
     const uint32_t per = (a.p.blocks + W - 1) / W, first = wave * per;
     const uint32_t end = first + per < a.p.blocks ? first + per : a.p.blocks;
     const uint32_t last_word = (a.p.cols - 1) & ~15u;
     const i32x4* w[RT];
+    const int8_t* x[NT];
 #pragma unroll
     for (int t = 0; t < RT; t++) {
         // Tiles past the last repeat it and are not stored.
         w[t] = reinterpret_cast<const i32x4*>(a.packed) +
             (size_t)(tile + t < a.p.tiles ? tile + t : a.p.tiles - 1) * a.p.blocks * 64 + lane;
     }
-    const int8_t* x = a.x + (token < a.tokens ? token : a.tokens - 1) * a.x_stride;
-    i32x4 wr[U][RT], xr[U], acc[RT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const uint32_t t = n * 16 + (lane & 15);
+        x[n] = a.x + (t < a.tokens ? t : a.tokens - 1) * a.x_stride;
+    }
+    i32x4 wr[U][RT], xr[U][NT], acc[RT][NT];
     auto load = [&](int u, uint32_t b) __attribute__((always_inline)) {
         // Words past the last column meet codes of 0.
         const uint32_t col = b * 64 + 16 * (lane >> 4);
-        xr[u] = *reinterpret_cast<const i32x4*>(x + (col < last_word ? col : last_word));
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            xr[u][n] = *reinterpret_cast<const i32x4*>(x[n] + (col < last_word ? col : last_word));
+        }
 #pragma unroll
         for (int t = 0; t < RT; t++) {
             wr[u][t] = __builtin_nontemporal_load(w[t] + (size_t)b * 64);
@@ -171,7 +181,10 @@ k_q8_few(Q8Args a)
     }
 #pragma unroll
     for (int t = 0; t < RT; t++) {
-        acc[t] = (i32x4){0, 0, 0, 0};
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            acc[t][n] = (i32x4){0, 0, 0, 0};
+        }
     }
     for (uint32_t b = first; b < end; b += U) {
 #pragma unroll
@@ -181,7 +194,11 @@ k_q8_few(Q8Args a)
             }
 #pragma unroll
             for (int t = 0; t < RT; t++) {
-                acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wr[u][t], xr[u], acc[t], 0, 0, 0);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    acc[t][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wr[u][t], xr[u][n],
+                        acc[t][n], 0, 0, 0);
+                }
             }
             if (b + u + U < end) {
                 load(u, b + u + U);
@@ -190,10 +207,14 @@ k_q8_few(Q8Args a)
     }
 #pragma unroll
     for (int t = 0; t < RT; t++) {
-        sums[wave][t][lane] = acc[t];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            sums[wave][t * NT + n][lane] = acc[t][n];
+        }
     }
     __syncthreads();
-    if (wave >= RT || token >= a.tokens || tile + wave >= a.p.tiles) {
+    const uint32_t token = wave % NT * 16 + (lane & 15), mine = tile + wave / NT;
+    if (wave >= RT * NT || token >= a.tokens || mine >= a.p.tiles) {
         return;
     }
     i32x4 v = sums[0][wave][lane];
@@ -201,7 +222,7 @@ k_q8_few(Q8Args a)
     for (int i = 1; i < W; i++) {
         v += sums[i][wave][lane];
     }
-    const uint32_t row = (tile + wave) * 16 + 4 * (lane >> 4);
+    const uint32_t row = mine * 16 + 4 * (lane >> 4);
     q8_put(a, q8_row_scales(a, row), v, token, a.x_scales[token], row, 0);
 }
 
@@ -463,7 +484,16 @@ extern "C" int lh_launch_q8_quantize(const float* w, uint32_t rows, uint32_t col
     return (int)hipGetLastError();
 }
 
-// Ways to run a product past 16 tokens: a workgroup's tile, the 1 / 64 us that a step takes
+// Whether k_q8_few runs a product: to 16 tokens, and to 32 where each workgroup's reading of
+// their words costs less than tiles in LDS, for few rows and columns: 6144 x 3072 for 24
+// tokens 7.4 us against 10.4, 3072 x 4096 7.0 against 8.6; but 3072 x 9216 for 32 12.2
+// against 9.8 (warm; cold 12.5 and 13.0 for 24), 18432 x 3072 18.7 against 16.3.
+static bool q8_few(uint32_t rows, uint32_t cols, uint32_t tokens)
+{
+    return tokens <= 16 || (tokens <= 32 && rows <= 12288 && cols <= 6144);
+}
+
+// Other ways to run a product: a workgroup's tile, the 1 / 64 us that a step takes
 // it where it is alone on a compute unit, and that it adds where others are there too.
 struct Q8Way {
     uint32_t rows, tokens, buffers, alone, shared;
@@ -472,7 +502,7 @@ static const Q8Way q8_ways[] = {
     {64, 32, 4, 13, 11}, {64, 64, 3, 18, 15}, {64, 128, 3, 24, 24}, {128, 128, 2, 46, 37},
     {192, 128, 2, 64, 50},
 };
-enum { Q8_WAYS = sizeof q8_ways / sizeof *q8_ways, Q8_SPLITS = 8, UNITS = 256, FEW_TOKENS = 16 };
+enum { Q8_WAYS = sizeof q8_ways / sizeof *q8_ways, Q8_SPLITS = 8, UNITS = 256 };
 
 struct Q8Plan {
     uint32_t way, splits, per;
@@ -526,7 +556,7 @@ static void q8_tiles(const Q8Args& a, hipStream_t s)
 
 extern "C" size_t lh_q8_scratch_bytes(uint32_t rows, uint32_t cols, uint32_t tokens)
 {
-    if (tokens <= FEW_TOKENS) {
+    if (q8_few(rows, cols, tokens)) {
         return 0;
     }
     const Q8Plan plan = q8_plan(rows, cols, tokens);
@@ -539,11 +569,13 @@ extern "C" int lh_launch_q8_matvec(const uint8_t* packed, const int8_t* x, size_
 {
     Q8Args a = {packed, q8_shape(rows, cols), x, x_scales, y, reinterpret_cast<int32_t*>(scratch),
         x_stride, y_stride, tokens, 1, 0};
-    if (tokens <= FEW_TOKENS) {
-        if (tokens > 4 && a.p.tiles >= 384) {
-            hipLaunchKernelGGL(k_q8_few<2>, dim3((a.p.tiles + 1) / 2), dim3(64 * FEW_WAVES), 0, s, a);
+    if (q8_few(rows, cols, tokens)) {
+        const uint32_t two = tokens > 4 && a.p.tiles >= 384;
+        const dim3 grid((a.p.tiles + two) / (1 + two)), block(64 * FEW_WAVES);
+        if (tokens <= 16) {
+            hipLaunchKernelGGL((two ? k_q8_few<2, 1> : k_q8_few<1, 1>), grid, block, 0, s, a);
         } else {
-            hipLaunchKernelGGL(k_q8_few<1>, dim3(a.p.tiles), dim3(64 * FEW_WAVES), 0, s, a);
+            hipLaunchKernelGGL((two ? k_q8_few<2, 2> : k_q8_few<1, 2>), grid, block, 0, s, a);
         }
         return (int)hipGetLastError();
     }
