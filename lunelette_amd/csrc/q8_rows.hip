@@ -165,10 +165,12 @@ k_q8_rows(lh_q8_source a)
     for (int q = 0; q < Q; q++) {
         load_h<KIND>(a, row, first + q * STEP, v[q]);
     }
-    float g[KIND == LH_Q8_NORM ? Q : 1][4], u[KIND == LH_Q8_SILU ? Q : 1][4];
+    // The norm's weights, from L2 a second time where registers do not hold them.
+    constexpr bool HELD = KIND == LH_Q8_NORM && Q <= 4;
+    float g[HELD ? Q : 1][4], u[KIND == LH_Q8_SILU ? Q : 1][4];
 #pragma unroll
     for (int q = 0; q < Q; q++) {
-        if (KIND == LH_Q8_NORM) {
+        if (HELD) {
             load_quad(a.gamma, first + q * STEP, a.width, g[q]);
         }
         if (KIND == LH_Q8_SILU) {
@@ -182,13 +184,17 @@ k_q8_rows(lh_q8_source a)
         if (KIND == LH_Q8_NORM && a.sum && c < a.width) {
             store_h(a, row, c, v[q]);
         }
+        float (&w)[4] = g[HELD ? q : 0];
+        if (KIND == LH_Q8_NORM && !HELD) {
+            load_quad(a.gamma, c, a.width, w);
+        }
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             if (KIND == LH_Q8_NORM) {
-                const double h = v[q][e], w = (double)g[q][e] * h;
+                const double h = v[q][e], value = (double)w[e] * h;
                 sum += h * h;
-                most = fmax(most, fabs(w));
-                bad |= !(fabs(w) <= 1e300);
+                most = fmax(most, fabs(value));
+                bad |= !(fabs(value) <= 1e300);
             } else if (KIND == LH_Q8_SILU) {
                 odd += v[q][e] * 0.0f + u[q][e] * 0.0f;
                 bad |= v[q][e] < -80.0f;   // 64 bits for the row
@@ -254,10 +260,14 @@ k_q8_rows(lh_q8_source a)
             continue;
         }
         int code[4] = {0, 0, 0, 0};
+        float (&weight)[4] = g[HELD ? q : 0];
+        if (KIND == LH_Q8_NORM && !HELD) {
+            load_quad(a.gamma, c, a.width, weight);
+        }
         if (fine && scale > 0) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float w = KIND == LH_Q8_NORM ? g[q][e] * v[q][e] : v[q][e];
+                const float w = KIND == LH_Q8_NORM ? weight[e] * v[q][e] : v[q][e];
                 const float t = w * by, n = rintf(t);
                 code[e] = (int)n;
                 const bool border = fabsf(fabsf(t - n) - 0.5f) < 0x1p-12f;
@@ -329,7 +339,7 @@ static void q8_rows(const lh_q8_source& a, hipStream_t s)
         dim3(64 * W * rows), 0, s, a);
 }
 
-// Few waves with up to four quads a lane: 3072 columns x 4096 tokens of the norm take four
+// Few waves with up to four quads a lane, where sixteen hold no row up to eight: 3072 columns x 4096 tokens of the norm take four
 // waves 33.4 us, twelve 34.8 (SwiGLU 25.8 and 39.6), 9216 x 2048 sixteen 58.1. Waves
 // that the four SIMDs do not share evenly take longer: three 37.1, nine 74.9.
 template <int KIND>
@@ -356,7 +366,15 @@ static void q8_rows(const lh_q8_source& a, hipStream_t s)
         q8_rows<KIND, 16, 3>(a, s);
     } else if (quads <= 64) {
         q8_rows<KIND, 16, 4>(a, s);
+    } else if (quads <= 96) {
+        q8_rows<KIND, 16, 6>(a, s);
     } else {
+        if constexpr (KIND != LH_Q8_NORM) {   // the norm's 64-bit values leave no registers
+            if (quads <= 128) {
+                q8_rows<KIND, 16, 8>(a, s);
+                return;
+            }
+        }
         hipLaunchKernelGGL(k_q8_wide_rows<KIND>, dim3(a.tokens), dim3(1024), 0, s, a);
     }
 }

@@ -98,7 +98,8 @@ def test_rows(gpu, tokens, width):
 
 
 @pytest.mark.parametrize("width", [w + d for w in (256, 512, 768, 1024, 2048, 3072, 4096, 6144, 8192,
-                                                  12288, 16384) for d in (-1, 0, 1)])
+                                                  12288, 16384, 24576, 32768)
+                                   for d in (-1, 0, 1)])
 def test_row_widths(gpu, width):
     """To either side of each way to hold a row, a number of rows that fills no workgroup."""
     rng = np.random.default_rng(width)
