@@ -92,7 +92,14 @@ struct Q8Args {
     uint32_t tokens, splits, per;   // per: 128-column steps of a split
 };
 
-// Sums v of rows row .. row + 3 for a token, as y or as a split's part. w: the rows' scales.
+// y of four rows' sums v for a token. w: the rows' scales.
+__device__ __forceinline__ float4 q8_values(float4 w, i32x4 v, float scale)
+{
+    return make_float4(scale * (w.x * (float)v[0]), scale * (w.y * (float)v[1]),
+        scale * (w.z * (float)v[2]), scale * (w.w * (float)v[3]));
+}
+
+// Sums v of rows row .. row + 3 for a token, as y or as a split's part.
 __device__ __forceinline__ void q8_put(const Q8Args& a, float4 w, i32x4 v, uint32_t token,
     float scale, uint32_t row, uint32_t split)
 {
@@ -102,8 +109,7 @@ __device__ __forceinline__ void q8_put(const Q8Args& a, float4 w, i32x4 v, uint3
         return;
     }
     float* y = a.y + token * a.y_stride + row;
-    const float4 r = make_float4(scale * (w.x * (float)v[0]), scale * (w.y * (float)v[1]),
-        scale * (w.z * (float)v[2]), scale * (w.w * (float)v[3]));
+    const float4 r = q8_values(w, v, scale);
     if (row + 3 < a.p.rows) {
         store4(y, r);
         return;
@@ -242,11 +248,12 @@ __device__ __forceinline__ void q8_meet()
 // of the columns. 128 columns (a step) of both operands at a time go to LDS as they are
 // multiplied, in B buffers: one is multiplied while the others fill.
 // Bound: at large tiles matrix instructions and the operands' way from L2 to LDS, which the
-// one barrier a step lets overlap in part. 18432 x 3072 for 2048 tokens takes 118 us, 1.97e15
-// operations a second, with cold inputs and outputs 130 (256 x 256 tiles: without the
+// one barrier a step lets overlap in part. 18432 x 3072 for 2048 tokens takes 120 us, 1.94e15
+// operations a second, with cold inputs and outputs 124 (256 x 256 tiles: without the
 // matrix instructions 100, without loads and reads 110, without stores 10 less, cold 20
 // less; the matrix instructions alone reach 3.5e15 to 4.1e15 on random codes).
-// Measured there, too: tiles of 192 x 256 in one workgroup a unit 115, cold 131, but 82
+// Measured there, too, with stores of 64 bytes of a row (123, cold 130): tiles of
+// 192 x 256 in one workgroup a unit 115, cold 131, but 82
 // against 77 for 1024 tokens and 94 against 78 for 3072 x 9216; 256 x 256 125, cold 139
 // (8192^3, which they fill: 2.37e15 a second); 128 x 256 in three buffers 144; workgroups
 // that go on to their next item 138 (registers); four waves of 96 x 128 172 (registers);
@@ -428,6 +435,36 @@ k_q8_tiles(Q8Args a, uint32_t mtiles, uint32_t ntiles)
     }
     __builtin_amdgcn_s_waitcnt(0x0f70);   // here: between stores it would wait for those too
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (MW >= 4) {
+        if (a.splits == 1 && (tile0 + MT) * 16 <= a.p.rows) {
+            // Through LDS, where all waves are done: a store then takes 256 bytes and more of a
+            // token's row in place of 64 (2048 tokens above 123 us -> 120, cold 130 -> 124).
+            constexpr int WIDE = MW * 16 + 4;   // floats of a token, in other banks than the next's
+            static_assert(W / 2 * 16 * WIDE * 4 <= SIZE, "half of the waves in a buffer");
+            __syncthreads();
+            float* mine = reinterpret_cast<float*>(wave < W / 2 ? buf0 : buf1) +
+                wave % (W / 2) * (16 * WIDE);
+            float* y = a.y + (tile0 + wm * MW) * 16;
+#pragma unroll
+            for (int n = 0; n < NW; n++) {
+#pragma unroll
+                for (int m = 0; m < MW; m++) {
+                    *reinterpret_cast<float4*>(mine + (lane & 15) * WIDE + m * 16 +
+                        4 * (lane >> 4)) = q8_values(w[m], acc[m][n], scale[n]);
+                }
+#pragma unroll
+                for (int i = 0; i < MW; i++) {
+                    const uint32_t t = (i * 64 + lane) / (MW * 4), c = (i * 64 + lane) % (MW * 4) * 4;
+                    const uint32_t token = token0 + (wn * NW + n) * 16 + t;
+                    const float4 v = *reinterpret_cast<const float4*>(mine + t * WIDE + c);
+                    if (token < a.tokens) {
+                        store4(y + token * a.y_stride + c, v);
+                    }
+                }
+            }
+            return;
+        }
+    }
 #pragma unroll
     for (int n = 0; n < NW; n++) {
         const uint32_t token = token0 + (wn * NW + n) * 16 + (lane & 15);
