@@ -2,6 +2,8 @@
 // best few tokens, for log probabilities (logprobs.hip) and beams (beam.hip).
 #pragma once
 
+#include <type_traits>
+
 #include "lh_device.h"
 
 namespace lh {
@@ -169,11 +171,15 @@ struct Candidates {
     uint32_t count;         // more than KEYS: the row needs the slow way
 };
 
-// The bound from the groups' largest; -Inf while fewer than `top` have any.
-__device__ __forceinline__ float group_bound(const volatile uint32_t* largest, uint32_t top,
+// The bound from the groups' largest; -Inf while fewer than `top` have any. An atomic load,
+// which stays a read of LDS: a volatile one waits for the chunks on their way too (256
+// rows of 131072 with 5 alternatives 30.4 us).
+__device__ __forceinline__ float group_bound(const uint32_t* largest, uint32_t top,
     uint32_t lane)
 {
-    const uint32_t rank = __builtin_amdgcn_readlane(sort_ranks(largest[lane], lane), 64 - top);
+    const uint32_t mine = __hip_atomic_load(&largest[lane], __ATOMIC_RELAXED,
+        __HIP_MEMORY_SCOPE_WORKGROUP);
+    const uint32_t rank = __builtin_amdgcn_readlane(sort_ranks(mine, lane), 64 - top);
     return rank ? rank_logit(rank) : -__builtin_inff();
 }
 
@@ -285,8 +291,10 @@ __device__ __forceinline__ void scan_part(PartShared& sh, const float* x, uint32
         some.count = 0;
     }
     __syncthreads();
-    for (uint32_t c = first; c < chunks || c == first; c += waves) {
-        const bool live = c < chunks;   // a wave without chunks comes for the barrier
+    // first_round: the one in which waves without chunks come for the barrier.
+    auto round = [&](uint32_t c, auto first_round) __attribute__((always_inline)) {
+        constexpr bool FIRST = decltype(first_round)::value;
+        const bool live = !FIRST || c < chunks;
         float v[16];
 #pragma unroll
         for (int i = 0; i < 16; i++) {
@@ -295,11 +303,15 @@ __device__ __forceinline__ void scan_part(PartShared& sh, const float* x, uint32
         if (c + waves < chunks) {
             load_chunk(x, vocab, c + waves, lane, next);
         }
-        float most = v[0];   // NaN if any is
+        float four[4], most;   // NaN if any is
 #pragma unroll
-        for (int i = 1; i < 16; i++) {
-            most = __builtin_elementwise_maximum(most, v[i]);
+        for (int q = 0; q < 4; q++) {
+            four[q] = __builtin_elementwise_maximum(
+                __builtin_elementwise_maximum(v[4 * q], v[4 * q + 1]),
+                __builtin_elementwise_maximum(v[4 * q + 2], v[4 * q + 3]));
         }
+        most = __builtin_elementwise_maximum(__builtin_elementwise_maximum(four[0], four[1]),
+            __builtin_elementwise_maximum(four[2], four[3]));
         bad |= !(most < __builtin_inff());
         const bool pass = top && __ballot(most >= bound);
         if (pass && most > -__builtin_inff()) {
@@ -318,17 +330,26 @@ __device__ __forceinline__ void scan_part(PartShared& sh, const float* x, uint32
                 r.w += (double)(e * d);
             }
         }
-        if (c == first && top) {
+        if (FIRST && top) {
             __syncthreads();   // the groups' largest of the whole first round
         }
         if (pass) {
             bound = group_bound(some.largest, top, lane);
             const uint32_t id = c * CHUNK + 4 * lane;
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                offer(some, v[i], id + 256 * (i >> 2) + (i & 3), bound);
+            for (int q = 0; q < 4; q++) {
+                if (__ballot(four[q] >= bound)) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        offer(some, v[4 * q + i], id + 256 * q + i, bound);
+                    }
+                }
             }
         }
+    };
+    round(first, std::true_type());
+    for (uint32_t c = first + waves; c < chunks; c += waves) {
+        round(c, std::false_type());
     }
     r.bad = __ballot(bad) != 0;
     r.z = wave_sum(r.z, lane);
