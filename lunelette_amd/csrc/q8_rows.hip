@@ -7,46 +7,62 @@
 // formed only where they decide: a quotient in FP32 is off by less than 2^-13, so
 // only one within 2^-12 of a border (one of 2000 to 4000) is formed again.
 // Bound: a row's bytes, read once into registers and written once. Measured: the norm with
-// the addition of 4096 rows of 3072 33.6 us, 4.9 TB/s (a large copy makes 4.7 to 5.2),
-// 4096 plain rows of 4096 16.2 us, 5.2 TB/s, SwiGLU of 2048 rows of 9216 45 us, 3.8 TB/s
-// (its exponential and two joins; with all of it in 64 bits 108); one row of the norm 4.1.
+// the addition of 4096 rows of 3072 33.0 us, 5.0 TB/s (a large copy makes 4.7 to 5.2),
+// 4096 plain rows of 4096 15.9 us, 5.3 TB/s, SwiGLU of 2048 rows of 9216 38.3 us, 4.4 TB/s
+// (its exponential and two joins; with all of it in 64 bits 108); one row of the norm 4.0.
 // A row in memory twice, and in 64 bits throughout, took the norm 77 us.
 #include "lh_serving.h"
 #include "lh_topk.h"
 
 namespace lh {
 
+// Over groups of 2 J lanes, the same bits in each.
 template <int J>
-__device__ __forceinline__ void join_lanes(double& sum, double& most, uint32_t lane)
+__device__ __forceinline__ double add_lanes(double v, uint32_t lane)
 {
-    sum += xor_double<J>(sum, lane);
-    most = fmax(most, xor_double<J>(most, lane));
+    v += xor_double<J>(v, lane);
     if constexpr (J > 1) {
-        join_lanes<J / 2>(sum, most, lane);
+        v = add_lanes<J / 2>(v, lane);
     }
+    return v;
 }
 
-// Sum and maximum (of values that are not NaN) over a row's W waves, in every lane. Each
-// call of a workgroup has `shared` of its own.
-template <int W>
-__device__ __forceinline__ void join_row(double& sum, double& most, double (&shared)[2][W],
+template <int J>
+__device__ __forceinline__ double most_lanes(double v, uint32_t lane)
+{
+    v = fmax(v, xor_double<J>(v, lane));
+    if constexpr (J > 1) {
+        v = most_lanes<J / 2>(v, lane);
+    }
+    return v;
+}
+
+template <int J>
+__device__ __forceinline__ float most_lanes(float v, uint32_t lane)
+{
+    v = fmaxf(v, __uint_as_float(xor_word<J>(__float_as_uint(v), lane)));
+    if constexpr (J > 1) {
+        v = most_lanes<J / 2>(v, lane);
+    }
+    return v;
+}
+
+// The maximum (of values that are not NaN) over a row's W waves and, if asked for, the sum,
+// in every lane. Each call of a workgroup has `shared` of its own.
+template <int W, bool SUM, typename T>
+__device__ __forceinline__ void join_row(double& sum, T& most, double (&shared)[2][W],
     uint32_t lane, uint32_t wave)
 {
-    join_lanes<32>(sum, most, lane);
-    if (W == 1) {
-        return;
-    }
-    if (lane == 0) {
-        shared[0][wave] = sum;
-        shared[1][wave] = most;
-    }
-    __syncthreads();
-    sum = shared[0][0];
-    most = shared[1][0];
-#pragma unroll
-    for (int i = 1; i < W; i++) {
-        sum += shared[0][i];
-        most = fmax(most, shared[1][i]);
+    sum = SUM ? add_lanes<32>(sum, lane) : sum;
+    most = most_lanes<32>(most, lane);
+    if constexpr (W > 1) {
+        if (lane == 0) {
+            shared[0][wave] = sum;
+            shared[1][wave] = most;
+        }
+        __syncthreads();
+        sum = SUM ? add_lanes<W / 2>(shared[0][lane % W], lane) : sum;
+        most = most_lanes<W / 2>((T)shared[1][lane % W], lane);
     }
 }
 
@@ -74,9 +90,10 @@ __device__ __forceinline__ double q8_wide(const lh_q8_source& a, size_t row, uin
     return KIND == LH_Q8_NORM ? (double)a.gamma[c] * (double)h * r : (double)h;
 }
 
-__device__ __forceinline__ int q8_code_wide(double v, float scale)
+// The code, its sign in the bits above.
+__device__ __forceinline__ uint32_t q8_code_wide(double v, float scale)
 {
-    return (int)rint(fmin(fmax(v / (double)scale, -127.0), 127.0));
+    return (uint32_t)(int)rint(fmin(fmax(v / (double)scale, -127.0), 127.0));
 }
 
 // Columns c .. c + 3 of a row; 0 past its end.
@@ -95,11 +112,13 @@ __device__ __forceinline__ void load_quad(const float* row, uint32_t c, uint32_t
 }
 
 __device__ __forceinline__ void store_codes(int8_t* to, uint32_t c, uint32_t width,
-    const int (&code)[4])
+    const uint32_t (&code)[4])
 {
     if (c + 3 < width) {
-        *reinterpret_cast<uint32_t*>(to + c) = (code[0] & 255) | (code[1] & 255) << 8 |
-            (code[2] & 255) << 16 | (uint32_t)code[3] << 24;
+        // Byte 0 of each: the second operand's bytes have indexes 0 to 3, the first's 4 to 7.
+        *reinterpret_cast<uint32_t*>(to + c) =
+            __builtin_amdgcn_perm(__builtin_amdgcn_perm(code[3], code[2], 0x0c0c0400u),
+                __builtin_amdgcn_perm(code[1], code[0], 0x0c0c0400u), 0x05040100u);
         return;
     }
 #pragma unroll
@@ -148,7 +167,7 @@ __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W)
 k_q8_rows(lh_q8_source a)
 {
     constexpr uint32_t ROWS = W == 1 ? 4 : 1, STEP = 256 * W;
-    __shared__ double shared[KIND == LH_Q8_SILU ? 3 : 1][ROWS][2][W];
+    __shared__ double shared[KIND == LH_Q8_SILU ? 2 : 1][ROWS][2][W];
     const uint32_t lane = threadIdx.x & 63;
     const uint32_t all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t wave = all % W, mine = all / W;
@@ -160,7 +179,6 @@ k_q8_rows(lh_q8_source a)
     float v[Q][4];
     double sum = 0, most = 0;
     bool bad = false;
-    float odd = 0;   // not 0: an Inf or NaN came in
 #pragma unroll
     for (int q = 0; q < Q; q++) {
         load_h<KIND>(a, row, first + q * STEP, v[q]);
@@ -177,10 +195,12 @@ k_q8_rows(lh_q8_source a)
             load_quad(a.second + row * a.second_stride, first + q * STEP, a.width, u[q]);
         }
     }
-    float near = 0;
+    // Largest magnitudes in FP32, NaN where there is one; the least gate.
+    float near = 0, quad[Q], least = 0;
 #pragma unroll
     for (int q = 0; q < Q; q++) {
         const uint32_t c = first + q * STEP;
+        quad[q] = 0;
         if (KIND == LH_Q8_NORM && a.sum && c < a.width) {
             store_h(a, row, c, v[q]);
         }
@@ -195,53 +215,51 @@ k_q8_rows(lh_q8_source a)
                 sum += h * h;
                 most = fmax(most, fabs(value));
                 bad |= !(fabs(value) <= 1e300);
-            } else if (KIND == LH_Q8_SILU) {
-                odd += v[q][e] * 0.0f + u[q][e] * 0.0f;
-                bad |= v[q][e] < -80.0f;   // 64 bits for the row
-                v[q][e] = silu_near(v[q][e], u[q][e]);
-                near = fmaxf(near, fabsf(v[q][e]));
             } else {
-                odd += v[q][e] * 0.0f;
-                near = fmaxf(near, fabsf(v[q][e]));
+                if (KIND == LH_Q8_SILU) {
+                    least = fminf(least, v[q][e]);
+                    v[q][e] = silu_near(v[q][e], u[q][e]);
+                }
+                quad[q] = __builtin_elementwise_maximum(quad[q], fabsf(v[q][e]));
             }
         }
+        near = __builtin_elementwise_maximum(near, quad[q]);
     }
     const double inf = __builtin_inf();
     double r = 1;
     bool wide = false;   // the whole row in 64 bits
     if (KIND == LH_Q8_NORM) {
         most = bad ? inf : most;
-        join_row<W>(sum, most, shared[0][mine], lane, wave);
+        join_row<W, true>(sum, most, shared[0][mine], lane, wave);
         wide = !(most >= 0x1p-90 && most < 0x1p120);
         r = 1.0 / sqrt(sum / a.width + 1e-5);
         most = sum < inf ? most * r : inf;   // a NaN too
     } else if (KIND == LH_Q8_ROWS) {
-        most = odd == 0 ? (double)near : inf;
-        join_row<W>(sum, most, shared[0][mine], lane, wave);
+        near = near < __builtin_inff() ? near : __builtin_inff();
+        join_row<W, false>(sum, near, shared[0][mine], lane, wave);
+        most = near;
     } else {
-        // First the largest in FP32 (-80 and below, Inf and NaN as larger ones still), then
-        // those near it in 64 bits.
-        sum = odd == 0 ? 0 : 1;
-        most = bad || !(near < 0x1p120f) ? 0x1p121 : (double)near;
-        join_row<W>(sum, most, shared[0][mine], lane, wave);
-        const bool none = sum != 0;
-        wide = !(most >= 0x1p-90 && most < 0x1p120);
-        const float from = (float)most * (1 - 0x1p-18f);
+        // First the largest in FP32 (beside gates below -80, an Inf or NaN a larger one still),
+        // then those near it in 64 bits. There an Inf or NaN gives one.
+        near = least >= -80.0f && near < 0x1p120f ? near : 0x1p121f;
+        join_row<W, false>(sum, near, shared[0][mine], lane, wave);
+        wide = !(near >= 0x1p-90f && near < 0x1p120f);
+        const float from = near * (1 - 0x1p-18f);
         most = 0;
-        if (!none) {
 #pragma unroll
-            for (int q = 0; q < Q; q++) {
+        for (int q = 0; q < Q; q++) {
+            if (wide || quad[q] >= from) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const uint32_t c = first + q * STEP + e;
-                    if (c < a.width && (wide || fabsf(v[q][e]) >= from)) {
-                        most = fmax(most, fabs(q8_wide<KIND>(a, row, c, 0, 1)));
+                    if ((wide || fabsf(v[q][e]) >= from) && c < a.width) {
+                        const double value = fabs(q8_wide<KIND>(a, row, c, 0, 1));
+                        most = fmax(most, value <= 1e300 ? value : inf);
                     }
                 }
             }
         }
-        join_row<W>(sum, most, shared[1][mine], lane, wave);
-        most = none ? inf : most;
+        join_row<W, false>(sum, most, shared[1][mine], lane, wave);
     }
     const float scale = (float)(most / 127.0);
     const bool fine = scale < __builtin_inff();
@@ -250,8 +268,13 @@ k_q8_rows(lh_q8_source a)
     }
     // v times this is the quotient, off by a few parts of 2^23; where that leaves FP32's
     // range all of the row takes 64 bits.
-    const float by = fine && scale > 0 ? (float)(r / (double)scale) : 0.0f;
+    const bool some = fine && scale > 0;
+    const float by = some ? (float)(r / (double)scale) : 0.0f;
     wide |= !(by >= 0x1p-100f && by <= 0x1p100f) || !(scale >= 0x1p-100f);
+    wide &= some;
+    // Added and taken away again it rounds to whole numbers, whose bits are then the lowest
+    // of the sum.
+    const float whole = 0x1.8p23f;
     int8_t* codes = a.codes + row * a.code_stride;
 #pragma unroll
     for (int q = 0; q < Q; q++) {
@@ -259,22 +282,27 @@ k_q8_rows(lh_q8_source a)
         if (c >= a.width) {
             continue;
         }
-        int code[4] = {0, 0, 0, 0};
         float (&weight)[4] = g[HELD ? q : 0];
         if (KIND == LH_Q8_NORM && !HELD) {
             load_quad(a.gamma, c, a.width, weight);
         }
-        if (fine && scale > 0) {
+        uint32_t code[4];
+        float off[4], most_off = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float w = KIND == LH_Q8_NORM ? weight[e] * v[q][e] : v[q][e];
+            const float t = w * by, rounded = t + whole;
+            code[e] = some ? __float_as_uint(rounded) : 0;
+            off[e] = fabsf(t - (rounded - whole));
+            most_off = fmaxf(most_off, off[e]);
+        }
+        const float border = 0.5f - 0x1p-12f;
+        if (wide || (some && most_off > border)) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float w = KIND == LH_Q8_NORM ? weight[e] * v[q][e] : v[q][e];
-                const float t = w * by, n = rintf(t);
-                code[e] = (int)n;
-                const bool border = fabsf(fabsf(t - n) - 0.5f) < 0x1p-12f;
-                if ((wide || border) && c + e < a.width) {
+                if ((wide || off[e] > border) && c + e < a.width) {
                     code[e] = q8_code_wide(q8_wide<KIND>(a, row, c + e, v[q][e], r), scale);
                 }
-                code[e] = code[e] < -127 ? -127 : code[e] > 127 ? 127 : code[e];
             }
         }
         store_codes(codes, c, a.width, code);
@@ -307,7 +335,7 @@ k_q8_wide_rows(lh_q8_source a)
         const double v = fabs(q8_wide<KIND>(a, row, c, h, 1));
         most = fmax(most, __builtin_isfinite(odd) && v <= 1e300 ? v : __builtin_inf());
     }
-    join_row<16>(sum, most, shared, lane, wave);
+    join_row<16, true>(sum, most, shared, lane, wave);
     const double r = KIND == LH_Q8_NORM ? 1.0 / sqrt(sum / a.width + 1e-5) : 1.0;
     const float scale = (float)(most * r / 127.0);
     const bool fine = scale < __builtin_inff();
@@ -316,7 +344,7 @@ k_q8_wide_rows(lh_q8_source a)
     }
     // The same thread's columns as before: a sum in place is its own.
     for (uint32_t c = threadIdx.x; c < a.width; c += 1024) {
-        int code = 0;
+        uint32_t code = 0;
         if (fine && scale > 0) {
             float h = 0;
             if (KIND == LH_Q8_NORM && a.sum) {
@@ -339,9 +367,10 @@ static void q8_rows(const lh_q8_source& a, hipStream_t s)
         dim3(64 * W * rows), 0, s, a);
 }
 
-// Few waves with up to four quads a lane, where sixteen hold no row up to eight: 3072 columns x 4096 tokens of the norm take four
-// waves 33.4 us, twelve 34.8 (SwiGLU 25.8 and 39.6), 9216 x 2048 sixteen 58.1. Waves
-// that the four SIMDs do not share evenly take longer: three 37.1, nine 74.9.
+// Few waves with up to four quads a lane, where sixteen hold no row up to eight: 4096 rows of
+// 3072 columns in four waves take 33.1 us (norm), 24.9 (SwiGLU) and 13.0 (plain), in twelve
+// with one quad 35.0, 34.1 and 17.9. Waves that the four SIMDs do not share evenly take
+// longer, three by 11%, nine by 29%.
 template <int KIND>
 static void q8_rows(const lh_q8_source& a, hipStream_t s)
 {
