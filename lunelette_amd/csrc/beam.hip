@@ -5,7 +5,7 @@
 // inside a row is that of its logit, so a row's best `keep` tokens by logit are all
 // that can be among the group's best. One pass over the logits, as for log
 // probabilities, gives every part of a row its range and its best tokens; a second
-// launch of a workgroup a group forms the scores in 64 bits and sorts the few of them
+// launch of a workgroup a group forms the scores in 64 bits and orders the few of them
 // that can be among the best.
 #include "lh_paged.h"
 #include "lh_serving.h"
@@ -81,8 +81,9 @@ __device__ __forceinline__ Place merge_places(Place best, Place rising, uint32_t
 }
 
 // LISTS: of a group, its beams' parts at most. PLACES: candidates that reach the group's
-// bound at most, `keep` of as many lists.
-enum { LISTS = 256, PLACES = LH_BEAMS * LH_BEAMS };
+// bound at most, `keep` of as many lists. FEW: candidates that are counted, not sorted.
+enum { LISTS = 256, PLACES = LH_BEAMS * LH_BEAMS, FEW = 128,
+    SHARE = FEW * FEW / (64 * WAVES) };
 
 struct BeamArgs {
     lh_beam_choice c;
@@ -126,7 +127,7 @@ k_beam_parts(BeamArgs a)
 struct BeamShared {
     double base[LH_BEAMS], log_z[LH_BEAMS];
     float most[LH_BEAMS];
-    uint32_t kind[LH_BEAMS], bad, count;
+    uint32_t kind[LH_BEAMS], bad, count, rank[FEW];
     Place bound, lists[WAVES][64];
     Place places[PLACES];
 };
@@ -221,7 +222,35 @@ k_beam_join(BeamArgs a)
     }
     Place p = {0, 0};
     uint32_t n = lists * c.keep;
-    if (n <= 64 * WAVES) {
+    const bool few = n <= FEW;
+    if (few) {
+        // A candidate's place is the number of better ones, counted by the waves in shares:
+        // the choice of 4 of 4 beams in both launches 11.7 us, sorted 13.4. The pairs of 256
+        // candidates take longer (14.5) than their sorting.
+        const uint32_t i = threadIdx.x % FEW, from = threadIdx.x / FEW * SHARE;
+        if (threadIdx.x < FEW) {
+            const uint32_t list = i / c.keep;
+            sh.rank[i] = 0;
+            sh.places[i] = i < n ? candidate(a, sh, row, list / a.parts, list % a.parts, i % c.keep)
+                : Place{0, 0};
+        } else if (wave == WAVES - 1) {
+            sh.lists[0][lane] = {0, 0};
+        }
+        __syncthreads();
+        const Place mine = sh.places[i];
+        uint32_t better = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < SHARE; j++) {
+            better += sh.places[from + j] > mine;
+        }
+        atomicAdd(&sh.rank[i], better);
+        __syncthreads();
+        if (threadIdx.x < FEW && mine.score && sh.rank[i] < c.keep) {
+            sh.lists[0][sh.rank[i]] = mine;
+        }
+        __syncthreads();
+        p = sh.lists[0][lane];
+    } else if (n <= 64 * WAVES) {
         // A candidate a thread.
         const uint32_t list = threadIdx.x / c.keep;
         if (threadIdx.x < n) {
@@ -257,7 +286,9 @@ k_beam_join(BeamArgs a)
                 : merge_places(p, sort_places(mine, lane, false), lane);
         }
     }
-    p = join_places(sh.lists, p, (n + 63) / 64 < WAVES ? (n + 63) / 64 : WAVES, wave, lane);
+    if (!few) {
+        p = join_places(sh.lists, p, (n + 63) / 64 < WAVES ? (n + 63) / 64 : WAVES, wave, lane);
+    }
     if (threadIdx.x < c.keep) {
         const size_t at = group * c.keep + threadIdx.x;
         const bool any = p.score != 0;
