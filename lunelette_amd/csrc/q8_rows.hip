@@ -161,6 +161,13 @@ __device__ __forceinline__ void store_h(const lh_q8_source& a, size_t row, uint3
     }
 }
 
+// Whether a maximum of magnitudes is below `to` and no NaN: by their bits, since the compiler
+// may take a chain of __builtin_elementwise_maximum for one without NaN.
+__device__ __forceinline__ bool below(float most, float to)
+{
+    return __float_as_uint(most) < __float_as_uint(to);
+}
+
 // A row in W waves, Q quads of columns a lane, all in registers.
 template <int KIND, int W, int Q>
 __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W)
@@ -235,13 +242,13 @@ k_q8_rows(lh_q8_source a)
         r = 1.0 / sqrt(sum / a.width + 1e-5);
         most = sum < inf ? most * r : inf;   // a NaN too
     } else if (KIND == LH_Q8_ROWS) {
-        near = near < __builtin_inff() ? near : __builtin_inff();
+        near = below(near, __builtin_inff()) ? near : __builtin_inff();
         join_row<W, false>(sum, near, shared[0][mine], lane, wave);
         most = near;
     } else {
         // First the largest in FP32 (beside gates below -80, an Inf or NaN a larger one still),
         // then those near it in 64 bits. There an Inf or NaN gives one.
-        near = least >= -80.0f && near < 0x1p120f ? near : 0x1p121f;
+        near = least >= -80.0f && below(near, 0x1p120f) ? near : 0x1p121f;
         join_row<W, false>(sum, near, shared[0][mine], lane, wave);
         wide = !(near >= 0x1p-90f && near < 0x1p120f);
         const float from = near * (1 - 0x1p-18f);

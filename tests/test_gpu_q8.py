@@ -185,6 +185,36 @@ def test_silu_ranges(gpu):
     assert list(np.nonzero(np.isnan(scales))[0]) == [2, 4, 5, 6, 7]
 
 
+@pytest.mark.parametrize("width", [200, 500, 700, 1001, 2000, 3000, 4000, 6000, 8000, 12000, 16001,
+                                   24000, 32000, 40000])
+def test_nonfinite_anywhere(gpu, width):
+    """One Inf or NaN in a row, in every part of it, in each input; the rows between stay."""
+    at = sorted({0, 3, 255, 256, width // 3, width // 2, 3 * width // 4, width - 2, width - 1}
+                & set(range(width)))
+    tokens = 2 * len(at) + 1
+    rng = np.random.default_rng(width)
+    x, second = (rng.normal(size=(tokens, width)).astype(np.float32) for _ in range(2))
+    gamma = rng.normal(size=width).astype(np.float32)
+    for odd in (np.float32(np.nan), np.float32(np.inf), np.float32(-np.inf)):
+        for place in (0, 1):
+            both = [x.copy(), second.copy()]
+            for i, c in enumerate(at):
+                both[place][2 * i + 1, c] = odd
+            bad = np.arange(tokens) % 2 == 1
+            h, v = q8.norm(both[0], both[1], gamma)
+            got = run_norm(gpu, both[0], both[1], gamma)
+            v[bad] = np.nan
+            q8.check_rows(*got[1:], v)
+            got = run_silu(gpu, *both)
+            v = q8.silu(*both)
+            v[bad] = np.nan
+            q8.check_rows(*got, v)
+            if not place:
+                got = run_rows(gpu, both[0])
+                q8.check_rows(*got, both[0].astype(np.float64))
+                assert np.array_equal(np.isnan(got[1]), bad) and not got[0][bad].any()
+
+
 @pytest.mark.parametrize("tokens,width", WIDTHS)
 def test_norm(gpu, tokens, width):
     rng = np.random.default_rng(tokens * 5 + width)
@@ -321,6 +351,29 @@ def test_quantized_weights(gpu):
     lh.check(gpu.lh_device_synchronize())
     want = q8.pack(gpu, codes, scales)
     assert np.array_equal(packed.download(np.uint32), want.download(np.uint32))
+
+
+@pytest.mark.parametrize("rows,cols", [(16, 5), (17, 1000), (3, 1500), (40, 2049)])
+def test_quantized_nonfinite_anywhere(gpu, rows, cols):
+    """One Inf or NaN in every other row, wherever it stands; packed codes from any address."""
+    rng = np.random.default_rng(rows * cols)
+    w = rng.normal(size=(rows, cols)).astype(np.float32)
+    for r in range(0, rows, 2):
+        w[r, r * (cols - 1) // max(1, rows - 1)] = (np.nan, np.inf, -np.inf)[r // 2 % 3]
+    codes, scales, _ = q8.quantize(w.astype(np.float64))
+    assert np.isnan(scales[::2]).all() and np.isfinite(scales[1::2]).all()
+    d_w = lh.DeviceBuffer.from_array(np.concatenate([np.zeros(1, np.float32), w.ravel()]))
+    d_s = lh.DeviceBuffer.from_array(scales)
+    packed = [lh.DeviceBuffer(gpu.lh_q8_bytes(rows, cols)) for _ in range(4)]
+    for p in packed:
+        lh.check(gpu.lh_memset_device(p.ptr, 0xff, p.nbytes))
+    lh.check(gpu.lh_q8_quantize(d_w.ptr + 4, rows, cols, packed[0].ptr, None))
+    for p, offset in zip(packed[1:], (0, 1, 7)):
+        d_c = lh.DeviceBuffer.from_array(np.concatenate([np.zeros(offset, np.int8), codes.ravel()]))
+        lh.check(gpu.lh_q8_pack(d_c.ptr + offset, d_s.ptr, rows, cols, p.ptr, None))
+        lh.check(gpu.lh_device_synchronize())
+    for p in packed[:1] + packed[2:]:
+        assert np.array_equal(p.download(np.uint8), packed[1].download(np.uint8))
 
 
 def test_matvec_large_offsets(gpu):
