@@ -90,6 +90,22 @@ def test_select(gpu, groups, beams, vocab, keep):
     check_choice(gpu, logits, scores, None, -1, keep, groups, beams)
 
 
+@pytest.mark.parametrize("beams,keep", [(1, 1), (2, 64), (64, 2), (3, 42), (3, 43), (43, 3), (16, 8),
+                                        (8, 17), (64, 3), (16, 64), (17, 64)])
+def test_select_numbers_of_candidates(gpu, beams, keep):
+    """To either side of 128 and of 1024 candidates in a group's lists, with equal logits in a
+    row, finished beams and beams without a score."""
+    rng = np.random.default_rng(beams * keep)
+    groups, vocab = 3, 900
+    n = groups * beams
+    logits = (np.round(8 * rng.normal(size=(n, vocab))) / 4).astype(np.float32)
+    scores = (-5 + 3 * rng.normal(size=n)).astype(np.float32)
+    check_choice(gpu, logits, scores, None, 7, keep, groups, beams)
+    done = rng.random(n) < 0.3
+    scores[rng.random(n) < 0.3] = -np.inf
+    check_choice(gpu, logits, scores, done, 7, keep, groups, beams)
+
+
 @pytest.mark.parametrize("vocab,keep", [(3000, 64), (70001, 20), (131072, 64), (515, 7)])
 def test_select_orders_ties_and_masks(gpu, vocab, keep):
     """Rows whose order is hard on a selection, one at a time in a group."""
