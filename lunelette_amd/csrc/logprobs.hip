@@ -12,8 +12,8 @@
 // of 1024 logits with the running maximum and the two sums and puts the few that may
 // be among the best `top` aside; both meet in the workgroup and, where a row has more
 // than one, in a second launch. Bound by the reads: 256 rows of 131072 with 5 alternatives
-// 31 us, 4.4 TB/s (28 us without any, 21 us for a plain read of as much); one row is
-// two launches and their memory round trips, 12 us.
+// 30 us, 4.4 TB/s (27 us without any, 21 us for a plain read of as much); one row is
+// two launches and their memory round trips, 11 us.
 #include "lh_serving.h"
 #include "lh_topk.h"
 
@@ -132,7 +132,7 @@ k_logprob_join(LogprobArgs a)
 
 using namespace lh;
 
-// Workgroups of a row: one for each unit of the chip in all (256 rows of 131072: 31 us;
+// Workgroups of a row: one for each unit of the chip in all (256 rows of 131072: 30 us;
 // with twice as many 42, a second launch and twice the candidates), each wave with a
 // chunk at least.
 enum { LOGPROB_WORKGROUPS = 256 };
