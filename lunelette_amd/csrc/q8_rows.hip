@@ -168,9 +168,11 @@ __device__ __forceinline__ bool below(float most, float to)
     return __float_as_uint(most) < __float_as_uint(to);
 }
 
-// A row in W waves, Q quads of columns a lane, all in registers.
+// A row in W waves, Q quads of columns a lane, all in registers. Sixteen waves with three quads
+// are held to 64 registers, so that a unit takes two rows at once: the norm of 2048 rows of
+// 9216, which would take 70, 50.2 us against 55.4.
 template <int KIND, int W, int Q>
-__global__ void __launch_bounds__(W == 1 ? 256 : 64 * W)
+__global__ void __launch_bounds__(W == 1 ? 256 : 64 * W, W == 16 && Q == 3 ? 8 : 1)
 k_q8_rows(lh_q8_source a)
 {
     constexpr uint32_t ROWS = W == 1 ? 4 : 1, STEP = 256 * W;
