@@ -157,6 +157,40 @@ def test_select_without_candidates(gpu):
     assert list(got[1][8]) == [777, -1, -1, -1, -1] and list(got[3][8]) == [1, 0, 0, 0, 0]
 
 
+@pytest.mark.parametrize("rows,vocab", [(256, 70001), (40, 131072), (9, 1500)])
+def test_a_nan_or_inf_anywhere_in_a_row(gpu, rows, vocab):
+    """The scan of a row, which log probabilities share, in every chunk and round of it."""
+    rng = np.random.default_rng(rows)
+    x = rng.normal(size=(rows, vocab)).astype(np.float32)
+    bad = np.arange(rows) % 5 != 0
+    for r in np.nonzero(bad)[0]:
+        x[r, r * (vocab - 1) // (rows - 1)] = (np.nan, np.inf)[r % 2]
+    x[::5, 1::2] = -np.inf
+    for keep in (1, 4, 64):
+        call = Choice(gpu, x, np.zeros(rows), None, -1, keep, rows, 1)
+        call.call()
+        parent, _, score, _ = call.get()
+        assert np.array_equal(np.isnan(score), np.repeat(bad[:, None], keep, 1))
+        assert np.array_equal(parent < 0, np.isnan(score))
+    d_x = lh.DeviceBuffer.from_array(x)
+    for top in (0, 4):
+        need = gpu.lh_logprobs_scratch(rows, vocab, top)
+        scratch = lh.DeviceBuffer(max(16, need))
+        tokens = lh.DeviceBuffer.from_array(np.zeros(rows, np.int64))
+        out = [lh.DeviceBuffer.from_array(np.zeros(rows, np.float32)) for _ in range(2)]
+        ids = lh.DeviceBuffer.from_array(np.zeros(rows * 4, np.int64))
+        best = lh.DeviceBuffer.from_array(np.zeros(rows * 4, np.float32))
+        lh.check(gpu.lh_logprobs(d_x.ptr, vocab, rows, vocab, tokens.ptr, out[0].ptr, out[1].ptr,
+                                 top, ids.ptr if top else None, best.ptr if top else None,
+                                 scratch.ptr, need, None))
+        lh.check(gpu.lh_device_synchronize())
+        for o in out:
+            assert np.array_equal(np.isnan(o.download(np.float32)), bad)
+        if top:
+            assert np.array_equal(ids.download(np.int64).reshape(rows, 4) < 0,
+                                  np.repeat(bad[:, None], 4, 1))
+
+
 def test_select_all_finished(gpu):
     rng = np.random.default_rng(10)
     logits = np.full((6, 9), np.nan, np.float32)
