@@ -66,8 +66,9 @@ __device__ __forceinline__ void join_row(double& sum, T& most, double (&shared)[
     }
 }
 
-// SiLU(g) * u with an error below 2^-20 of itself, for g above -80 and results between
-// 2^-90 and 2^120.
+// SiLU(g) * u with an error below 2^-20 of itself or of 2^-60, for g above -80, |u| below
+// 2^66 and results below 2^120. (Where g times the factor is subnormal it loses up to
+// 2^-150, of which u makes 2^-84; the factor itself is no less than 2^-117.)
 __device__ __forceinline__ float silu_near(float g, float u)
 {
     const float e = exp_near(-fabsf(g)), part = __builtin_amdgcn_rcpf(1.0f + e);
@@ -204,8 +205,8 @@ k_q8_rows(lh_q8_source a)
             load_quad(a.second + row * a.second_stride, first + q * STEP, a.width, u[q]);
         }
     }
-    // Largest magnitudes in FP32, NaN where there is one; the least gate.
-    float near = 0, quad[Q], least = 0;
+    // Largest magnitudes in FP32, NaN where there is one; the least gate, the largest up.
+    float near = 0, quad[Q], least = 0, most_up = 0;
 #pragma unroll
     for (int q = 0; q < Q; q++) {
         const uint32_t c = first + q * STEP;
@@ -227,6 +228,7 @@ k_q8_rows(lh_q8_source a)
             } else {
                 if (KIND == LH_Q8_SILU) {
                     least = fminf(least, v[q][e]);
+                    most_up = fmaxf(most_up, fabsf(u[q][e]));
                     v[q][e] = silu_near(v[q][e], u[q][e]);
                 }
                 quad[q] = __builtin_elementwise_maximum(quad[q], fabsf(v[q][e]));
@@ -248,11 +250,12 @@ k_q8_rows(lh_q8_source a)
         join_row<W, false>(sum, near, shared[0][mine], lane, wave);
         most = near;
     } else {
-        // First the largest in FP32 (beside gates below -80, an Inf or NaN a larger one still),
-        // then those near it in 64 bits. There an Inf or NaN gives one.
-        near = least >= -80.0f && below(near, 0x1p120f) ? near : 0x1p121f;
+        // First the largest in FP32 (beside what silu_near does not take, an Inf or NaN a larger
+        // one still), then those near it in 64 bits. There an Inf or NaN gives one.
+        const bool taken = least >= -80.0f && most_up < 0x1p66f && below(near, 0x1p120f);
+        near = taken ? near : 0x1p121f;
         join_row<W, false>(sum, near, shared[0][mine], lane, wave);
-        wide = !(near >= 0x1p-90f && near < 0x1p120f);
+        wide = !(near >= 0x1p-60f && near < 0x1p120f);
         const float from = near * (1 - 0x1p-18f);
         most = 0;
 #pragma unroll
