@@ -45,6 +45,8 @@ int lh_launch_q8_quantize(const float *w, uint32_t rows, uint32_t cols, uint8_t 
 int lh_launch_q8_matvec(const uint8_t *packed, const int8_t *x, size_t x_stride,
     const float *x_scales, float *y, size_t y_stride, uint32_t rows, uint32_t cols,
     uint32_t tokens, uint8_t *scratch, hipStream_t s);
+/* The kernel that lh_launch_q8_matvec takes at these sizes, and its column splits. */
+int lh_q8_way(uint32_t rows, uint32_t cols, uint32_t tokens, uint32_t *splits);
 
 int lh_launch_logprobs(const float *logits, size_t stride, uint32_t rows, uint32_t vocab,
     const int64_t *tokens, float *logprob, float *entropy, uint32_t top, int64_t *top_ids,

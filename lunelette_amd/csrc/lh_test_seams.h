@@ -37,6 +37,10 @@ int lunelette_metal_test_chained(uint32_t length);
 /* The matrix-core attention's KV splits for count tokens after length positions;
  * 1 when the long-prefix kernel runs, 0 otherwise. */
 int lunelette_metal_test_attention_plan(uint32_t length, uint32_t count, uint32_t *splits);
+/* The kernel of an lh_q8_matvec of these sizes: 0..3 the streamed weights' (two tiles
+ * of rows a workgroup 1, two of tokens 2), from 4 on the tiles in LDS, in the order
+ * of their sizes; and the number of its column splits. */
+int lunelette_metal_test_q8_way(uint32_t rows, uint32_t cols, uint32_t tokens, uint32_t *splits);
 /* Overwrites one published host logit. */
 int lunelette_metal_test_set_logit(struct lunelette_metal *context, size_t index, float value);
 /* Arms the allocation counter: the nth device or pinned-host allocation from

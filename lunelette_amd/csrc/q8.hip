@@ -620,6 +620,19 @@ static Q8Plan q8_plan(uint32_t rows, uint32_t cols, uint32_t tokens)
     return best;
 }
 
+// The kernel that a product runs: k_q8_few with two tiles of rows (1) or not (0), with two
+// of tokens (2 more), or from 4 on one of q8_ways.
+static Q8Plan q8_kernel(uint32_t rows, uint32_t cols, uint32_t tokens)
+{
+    if (q8_few(rows, cols, tokens)) {
+        const bool two = tokens > 4 && (rows + 15) / 16 >= 384;
+        return {two + 2u * (tokens > 16), 1, 0};
+    }
+    Q8Plan plan = q8_plan(rows, cols, tokens);
+    plan.way += 4;
+    return plan;
+}
+
 template <int MW, int NW, int WM, int WN, int B>
 static void q8_tiles(const Q8Args& a, hipStream_t s)
 {
@@ -629,39 +642,43 @@ static void q8_tiles(const Q8Args& a, hipStream_t s)
         0, s, a, m, n);
 }
 
+template <int RT, int NT>
+static void q8_streamed(const Q8Args& a, hipStream_t s)
+{
+    hipLaunchKernelGGL((k_q8_few<RT, NT>), dim3((a.p.tiles + RT - 1) / RT), dim3(64 * FEW_WAVES),
+        0, s, a);
+}
+
+extern "C" int lh_q8_way(uint32_t rows, uint32_t cols, uint32_t tokens, uint32_t* splits)
+{
+    const Q8Plan plan = q8_kernel(rows, cols, tokens);
+    *splits = plan.splits;
+    return (int)plan.way;
+}
+
 extern "C" size_t lh_q8_scratch_bytes(uint32_t rows, uint32_t cols, uint32_t tokens)
 {
-    if (q8_few(rows, cols, tokens)) {
-        return 0;
-    }
-    const Q8Plan plan = q8_plan(rows, cols, tokens);
-    return plan.splits == 1 ? 0 : (size_t)plan.splits * tokens * ((rows + 15) / 16 * 64);
+    uint32_t splits;
+    lh_q8_way(rows, cols, tokens, &splits);
+    return splits == 1 ? 0 : (size_t)splits * tokens * ((rows + 15) / 16 * 64);
 }
 
 extern "C" int lh_launch_q8_matvec(const uint8_t* packed, const int8_t* x, size_t x_stride,
     const float* x_scales, float* y, size_t y_stride, uint32_t rows, uint32_t cols,
     uint32_t tokens, uint8_t* scratch, hipStream_t s)
 {
-    Q8Args a = {packed, q8_shape(rows, cols), x, x_scales, y, reinterpret_cast<int32_t*>(scratch),
-        x_stride, y_stride, tokens, 1, 0};
-    if (q8_few(rows, cols, tokens)) {
-        const uint32_t two = tokens > 4 && a.p.tiles >= 384;
-        const dim3 grid((a.p.tiles + two) / (1 + two)), block(64 * FEW_WAVES);
-        if (tokens <= 16) {
-            hipLaunchKernelGGL((two ? k_q8_few<2, 1> : k_q8_few<1, 1>), grid, block, 0, s, a);
-        } else {
-            hipLaunchKernelGGL((two ? k_q8_few<2, 2> : k_q8_few<1, 2>), grid, block, 0, s, a);
-        }
-        return (int)hipGetLastError();
-    }
-    const Q8Plan plan = q8_plan(rows, cols, tokens);
-    a.splits = plan.splits;
-    a.per = plan.per;
+    const Q8Plan plan = q8_kernel(rows, cols, tokens);
+    const Q8Args a = {packed, q8_shape(rows, cols), x, x_scales, y,
+        reinterpret_cast<int32_t*>(scratch), x_stride, y_stride, tokens, plan.splits, plan.per};
     switch (plan.way) {
-    case 0: q8_tiles<1, 2, 4, 1, 4>(a, s); break;
-    case 1: q8_tiles<2, 2, 2, 2, 3>(a, s); break;
-    case 2: q8_tiles<2, 2, 2, 4, 3>(a, s); break;
-    case 3: q8_tiles<4, 2, 2, 4, 2>(a, s); break;
+    case 0: q8_streamed<1, 1>(a, s); break;
+    case 1: q8_streamed<2, 1>(a, s); break;
+    case 2: q8_streamed<1, 2>(a, s); break;
+    case 3: q8_streamed<2, 2>(a, s); break;
+    case 4: q8_tiles<1, 2, 4, 1, 4>(a, s); break;
+    case 5: q8_tiles<2, 2, 2, 2, 3>(a, s); break;
+    case 6: q8_tiles<2, 2, 2, 4, 3>(a, s); break;
+    case 7: q8_tiles<4, 2, 2, 4, 2>(a, s); break;
     default: q8_tiles<6, 4, 2, 2, 2>(a, s); break;
     }
     const hipError_t e = hipGetLastError();

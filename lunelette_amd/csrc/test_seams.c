@@ -3,6 +3,7 @@
 #include "lh_test_seams.h"
 #include "lh_internal.h"
 #include "lh_host_alloc.h"
+#include "lh_serving.h"
 
 int lunelette_metal_test_inject(struct lunelette_metal *context, int what)
 {
@@ -66,4 +67,9 @@ int lunelette_metal_test_chained(uint32_t length)
 int lunelette_metal_test_attention_plan(uint32_t length, uint32_t count, uint32_t *splits)
 {
     return lh_attention_mfma_plan(length, count, splits);
+}
+
+int lunelette_metal_test_q8_way(uint32_t rows, uint32_t cols, uint32_t tokens, uint32_t *splits)
+{
+    return lh_q8_way(rows, cols, tokens, splits);
 }
