@@ -280,6 +280,15 @@ __device__ __forceinline__ void q8_meet()
     asm volatile("" ::: "memory");
 }
 
+// A wave's own barrier: its lanes' accesses to LDS (which the unit makes in the order of the
+// program) stay to their side of it.
+__device__ __forceinline__ void wave_meet()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // The product of many tokens. A workgroup of WM x WN waves forms the sums of MT = WM * MW
 // tiles of rows and NT = WN * NW tiles of tokens, a wave MW x NW of them, over a split
 // of the columns. 128 columns (a step) of both operands at a time go to LDS as they are
@@ -489,6 +498,7 @@ k_q8_tiles(Q8Args a, uint32_t mtiles, uint32_t ntiles)
                     *reinterpret_cast<float4*>(mine + (lane & 15) * WIDE + m * 16 +
                         4 * (lane >> 4)) = q8_values(w[m], acc[m][n], scale[n]);
                 }
+                wave_meet();
 #pragma unroll
                 for (int i = 0; i < MW; i++) {
                     const uint32_t t = (i * 64 + lane) / (MW * 4);
@@ -499,6 +509,7 @@ k_q8_tiles(Q8Args a, uint32_t mtiles, uint32_t ntiles)
                         store4(y + token * a.y_stride + c, v);
                     }
                 }
+                wave_meet();
             }
             return;
         }
