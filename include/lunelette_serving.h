@@ -210,7 +210,7 @@ int lh_paged_attention(const lh_paged_cache *cache, const lh_paged_batch *batch,
 
 #define LH_BEAMS 64   /* of a group, and places that a group keeps */
 
-/* Scratch bytes of lh_beam_select (0: none is needed, or sizes that it refuses). */
+/* Scratch bytes of lh_beam_select; 0 for sizes that it refuses. */
 size_t lh_beam_scratch(size_t groups, size_t beams, size_t vocab, size_t keep);
 /* The best continuations of each group's beams. A beam of score s (d_scores
  * [groups * beams], FP32) has a candidate of score s + ln p for each token of its
@@ -225,8 +225,13 @@ size_t lh_beam_scratch(size_t groups, size_t beams, size_t vocab, size_t keep);
  * Places past a group's candidates hold parent -1, token -1, score -Inf, done 0. Where
  * a beam's score is NaN or +Inf, or the row of one that is read holds a NaN or
  * +Inf, all places of its group hold parent -1, token -1, score NaN, done 0.
- * groups * beams 1..65535, beams 1..LH_BEAMS, vocab 1..2^24, stride >= vocab. The
- * sums are formed in 64 bits. Outputs share no element with inputs. */
+ * groups * beams 1..65535, beams 1..LH_BEAMS, vocab 1..2^24, stride >= vocab.
+ * Outputs share no element with inputs.
+ * Scores are 64-bit sums, but a row's ln Z (ln p = logit - ln Z) comes of exponentials
+ * in FP32, added in 64 bits: it is off by up to (ln vocab + 8) 2^-24 (1.2e-6 for 131072
+ * tokens). That moves all of a beam's candidates alike, so only those of different beams
+ * can change places, where their scores are nearer than twice that; and as the number of
+ * parts that a row is added up in depends on groups * beams, so may such an order. */
 int lh_beam_select(const float *d_logits, size_t stride, size_t groups, size_t beams,
     size_t vocab, const float *d_scores, const uint8_t *d_done, int64_t stop, size_t keep,
     int32_t *d_parent, int64_t *d_token, float *d_score, uint8_t *d_done_out, void *d_scratch,
