@@ -80,10 +80,9 @@ __device__ __forceinline__ Place merge_places(Place best, Place rising, uint32_t
     return half_merge<32>(best > rising ? best : rising, lane, true);
 }
 
-// LISTS: of a group, its beams' parts at most. PLACES: candidates that reach the group's
-// bound at most, `keep` of as many lists. FEW: candidates that are counted, not sorted.
-enum { LISTS = 256, PLACES = LH_BEAMS * LH_BEAMS, FEW = 128,
-    SHARE = FEW * FEW / (64 * WAVES) };
+// PLACES: candidates that reach the group's bound at most, `keep` of as many lists. FEW:
+// candidates that are counted, not sorted.
+enum { PLACES = LH_BEAMS * LH_BEAMS, FEW = 128, SHARE = FEW * FEW / (64 * WAVES) };
 
 struct BeamArgs {
     lh_beam_choice c;
@@ -259,7 +258,8 @@ k_beam_join(BeamArgs a)
         p = sort_places(p, lane, true);
     } else {
         // Lists are falling, so the keep-th best of their first places bounds the group's best
-        // from below, and only `keep` lists reach it. A list a lane of the first four waves.
+        // from below, and only `keep` lists reach it. A list a lane of the first four waves:
+        // a group has 256 at most (beam_parts).
         if (threadIdx.x < lists) {
             p = candidate(a, sh, row, threadIdx.x / a.parts, threadIdx.x % a.parts, 0);
         }
@@ -360,7 +360,7 @@ __device__ __forceinline__ uint32_t open_column(const ReorderArgs& a, int32_t le
 // that are copied, then the sequences' rows. No page is both read and written: the pages
 // read stay their first child's, those written belong to beams without children.
 // Bound: the pages' bytes; 8 groups of 8 beams in FP16 pages of 26 layers (436 MB
-// both ways) 67 us, 6.5 TB/s; 4 beams in 4-bit pages 4.3 us, the loads of parents, length,
+// both ways) 74 us, 5.9 TB/s; 4 beams in 4-bit pages 4.5 us, the loads of parents, length,
 // page ids and page one after another.
 __global__ void __launch_bounds__(256)
 k_beam_copy(ReorderArgs a)
@@ -401,7 +401,7 @@ k_beam_copy(ReorderArgs a)
 }
 
 // grid (column tiles, groups): rows of tables in place. All of a group are read before one
-// is written.
+// is written. A launch after the copies' takes 3.4 us (4 beams above 7.9 in all) to 5.3 (79).
 __global__ void __launch_bounds__(256)
 k_beam_tables(ReorderArgs a)
 {
@@ -436,7 +436,7 @@ k_beam_tables(ReorderArgs a)
 using namespace lh;
 
 // Workgroups of a row, as for log probabilities: one for each unit of the chip in all, each
-// wave with a chunk at least.
+// wave with a chunk at least. A group's beams have 256 together, or one each.
 static uint32_t beam_parts(uint32_t rows, uint32_t vocab)
 {
     const uint32_t chunks = (vocab + CHUNK - 1) / CHUNK, most = (chunks + WAVES - 1) / WAVES;

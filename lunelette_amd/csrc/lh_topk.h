@@ -312,6 +312,8 @@ __device__ __forceinline__ void scan_part(PartShared& sh, const float* x, uint32
         }
         most = __builtin_elementwise_maximum(__builtin_elementwise_maximum(four[0], four[1]),
             __builtin_elementwise_maximum(four[2], four[3]));
+        // Each lane for itself: in a vote over `most < infinity` the compiler would compare for
+        // `not equal` to it, which a NaN passes.
         bad |= !(most < __builtin_inff());
         const bool pass = top && __ballot(most >= bound);
         if (pass && most > -__builtin_inff()) {

@@ -12,7 +12,7 @@
 // of 1024 logits with the running maximum and the two sums and puts the few that may
 // be among the best `top` aside; both meet in the workgroup and, where a row has more
 // than one, in a second launch. Bound by the reads: 256 rows of 131072 with 5 alternatives
-// 30 us, 4.4 TB/s (27 us without any, 21 us for a plain read of as much); one row is
+// 28.5 us, 4.7 TB/s (27 us without any, 21 us for a plain read of as much); one row is
 // two launches and their memory round trips, 11 us.
 #include "lh_serving.h"
 #include "lh_topk.h"

@@ -78,8 +78,8 @@ k_q8_quantize(const float* __restrict__ w, Q8Shape p, uint8_t* __restrict__ pack
     const uint32_t tile = blockIdx.x, row = tile * 16 + in;
     const float* x = w + (size_t)row * p.cols;
     const uint32_t cols = row < p.rows ? p.cols : 0;
-    // Magnitudes as whole numbers, among which Inf and NaN are the largest. (A loop over
-    // __builtin_elementwise_maximum is taken by the compiler for one without NaN.)
+    // Magnitudes as whole numbers, among which Inf and NaN are the largest. (The compiler forms a
+    // vote over `v < infinity` with a comparison that a NaN passes: not equal to it.)
     uint32_t most = 0;
 #pragma unroll 4
     for (uint32_t c = 4 * lane; c < cols; c += 256) {
@@ -169,13 +169,10 @@ __device__ __forceinline__ float4 q8_row_scales(const Q8Args& a, uint32_t row)
 // eight waves a slice of the columns each; a wave asks for U blocks of its slice at once
 // and for another whenever it has multiplied one. The sums meet in LDS.
 // Bound: the weights' bytes. Measured, cold weights: 18432 x 3072 (57 MB) for one token
-// 10.4 us, 5.4 TB/s, 131072 x 3072 for eight 59 us, 6.8 TB/s; 3072 x 9216 6.7 us, of
+// 10.5 us, 5.4 TB/s, 131072 x 3072 for eight 62 us, 6.5 TB/s; 3072 x 9216 6.8 us, of
 // which a launch and the first bytes' way are 4. More tokens' words are 16 rows apart each,
-// which a request takes half a cache line of: 3072 x 9216 for 16 tokens 10.2 us. Two tiles
-// of rows share them where there are workgroups enough: 18432 x 3072 for 16 tokens 14.0
-// us (one tile 14.7), 6144 x 3072 for eight 5.7 (6.2), for 24 7.4 (9.2); but for one token
-// 11.8 (10.4), and 3072 x 9216 for 16 12.7. Nine blocks on their way or three, sixteen
-// waves or four: no gain.
+// which a request takes half a cache line of: 3072 x 9216 for 16 tokens 10.3 us. Nine
+// blocks on their way or three, sixteen waves or four: no gain.
 enum { FEW_WAVES = 8 };
 
 template <int RT, int NT>
@@ -294,8 +291,10 @@ __device__ __forceinline__ void wave_meet()
 // of the columns. 128 columns (a step) of both operands at a time go to LDS as they are
 // multiplied, in B buffers: one is multiplied while the others fill.
 // Bound: at large tiles matrix instructions and the operands' way from L2 to LDS, which the
-// one barrier a step lets overlap in part. 18432 x 3072 for 2048 tokens takes 120 us, 1.94e15
-// operations a second, with cold inputs and outputs 124 (256 x 256 tiles: without the
+// one barrier a step lets overlap in part. 18432 x 3072 for 2048 tokens takes 115 us, 2.0e15
+// operations a second, with cold weights 122, with cold inputs and outputs too 124, and 134 to
+// 139 beside a profiler. The figures below are of an earlier box, where it took 116 and, all
+// cold, 124 (256 x 256 tiles: without the
 // matrix instructions 100, without loads and reads 110, without stores 10 less, cold 20
 // less; the matrix instructions alone reach 3.5e15 to 4.1e15 on random codes).
 // Measured there, too, with stores of 64 bytes of a row (123, cold 130): tiles of
@@ -484,7 +483,7 @@ k_q8_tiles(Q8Args a, uint32_t mtiles, uint32_t ntiles)
     if constexpr (MW >= 4) {
         if (a.splits == 1 && (tile0 + MT) * 16 <= a.p.rows) {
             // Through LDS, where all waves are done: a store then takes 256 bytes and more of a
-            // token's row in place of 64 (2048 tokens above 123 us -> 120, cold 130 -> 124).
+            // token's row in place of 64 (2048 tokens above 123 us -> 116, cold 130 -> 124).
             constexpr int WIDE = MW * 16 + 4;   // floats of a token, in other banks than the next's
             static_assert(W / 2 * 16 * WIDE * 4 <= SIZE, "half of the waves in a buffer");
             __syncthreads();
@@ -571,9 +570,14 @@ extern "C" int lh_launch_q8_quantize(const float* w, uint32_t rows, uint32_t col
 }
 
 // Whether k_q8_few runs a product: to 16 tokens, and to 32 where each workgroup's reading of
-// their words costs less than tiles in LDS, for few rows and columns: 6144 x 3072 for 24
-// tokens 7.4 us against 10.4, 3072 x 4096 7.0 against 8.6; but 3072 x 9216 for 32 12.2
-// against 9.8 (warm; cold 12.5 and 13.0 for 24), 18432 x 3072 18.7 against 16.3.
+// their words costs less than tiles in LDS, for few rows and columns. Measured (17, 24, 32
+// tokens, cold weights, us; tiles in brackets):
+//   3072 x 3072     5.3  6.0  6.6 ( 8.3  8.7  9.1)   3072 x 6144   8.4  9.7 11.0 (10.5 10.7 11.0)
+//   6144 x 3072     6.7  7.5  8.2 (10.7 10.8 10.9)   6144 x 6144  11.1 12.3 13.9 (12.8 13.0 13.6)
+//   12288 x 3072   10.6 11.9 13.4 (11.6 11.7 11.8)   3072 x 9216  10.7 12.6 14.3 (12.6 12.9 12.9)
+//   18432 x 3072   14.5 16.4 18.6 (15.2 15.7 16.3)   1024 x 16384 15.0 17.8 21.0 (12.2 12.5 12.7)
+// The limits are those of 24 tokens; 17 tokens would gain 5 to 15% past them, 32 lose as much
+// within (12288 x 6144: 24.2 against 20.2).
 static bool q8_few(uint32_t rows, uint32_t cols, uint32_t tokens)
 {
     return tokens <= 16 || (tokens <= 32 && rows <= 12288 && cols <= 6144);
@@ -633,6 +637,12 @@ static Q8Plan q8_plan(uint32_t rows, uint32_t cols, uint32_t tokens)
 
 // The kernel that a product runs: k_q8_few with two tiles of rows (1) or not (0), with two
 // of tokens (2 more), or from 4 on one of q8_ways.
+// Two tiles of rows share the tokens' words, but leave half the workgroups. Measured, one tile
+// against two (us, cold weights): 6144 x 3072 for 4 tokens 5.8 and 5.6, for 8 6.3 and 5.8, for
+// 16 7.6 and 6.6, for 24 9.3 and 7.6; 12288 x 3072 for 24 16.0 and 12.0; 131072 x 3072 for 4
+// 57.6 and 59.7, for 8 62.7 and 61.7, for 16 89 and 72; below 384 tiles, 4096 x 3072 for 16 5.4
+// and 6.3. Not on its side are few tokens over many rows: 18432 x 3072 for 5 to 12 10.8 to 12.9
+// and 13.0 to 14.4 (16: 14.7 and 14.4), 8192 x 8192 for 8 13.1 and 15.8.
 static Q8Plan q8_kernel(uint32_t rows, uint32_t cols, uint32_t tokens)
 {
     if (q8_few(rows, cols, tokens)) {

@@ -7,10 +7,11 @@
 // formed only where they decide: a quotient in FP32 is off by less than 2^-13, so
 // only one within 2^-12 of a border (one of 2000 to 4000) is formed again.
 // Bound: a row's bytes, read once into registers and written once. Measured: the norm with
-// the addition of 4096 rows of 3072 33.0 us, 5.0 TB/s (a large copy makes 4.7 to 5.2),
-// 4096 plain rows of 4096 15.9 us, 5.3 TB/s, SwiGLU of 2048 rows of 9216 38.3 us, 4.4 TB/s
-// (its exponential and two joins; with all of it in 64 bits 108); one row of the norm 4.0.
-// A row in memory twice, and in 64 bits throughout, took the norm 77 us.
+// the addition of 4096 rows of 3072 32.6 us, 5.0 TB/s (a large copy makes 4.7 to 5.2),
+// 4096 plain rows of 4096 15.8 us, 5.3 TB/s, SwiGLU of 2048 rows of 9216 38.7 us, 4.4 TB/s
+// (its exponential and two joins); one row of the norm 4.0. A row in memory twice, and in
+// 64 bits throughout, took the norm 77 us. Rows that FP32 does not decide are in 64 bits
+// here as well: SwiGLU with a gate below -80 in each row 106 us.
 #include "lh_serving.h"
 #include "lh_topk.h"
 
@@ -162,8 +163,8 @@ __device__ __forceinline__ void store_h(const lh_q8_source& a, size_t row, uint3
     }
 }
 
-// Whether a maximum of magnitudes is below `to` and no NaN: by their bits, since the compiler
-// may take a chain of __builtin_elementwise_maximum for one without NaN.
+// Whether a maximum of magnitudes is below `to` and no NaN: by their bits, which are above
+// infinity's for a NaN.
 __device__ __forceinline__ bool below(float most, float to)
 {
     return __float_as_uint(most) < __float_as_uint(to);
