@@ -293,8 +293,7 @@ __device__ __forceinline__ void wave_meet()
 // Bound: at large tiles matrix instructions and the operands' way from L2 to LDS, which the
 // one barrier a step lets overlap in part. 18432 x 3072 for 2048 tokens takes 115 us, 2.0e15
 // operations a second, with cold weights 122, with cold inputs and outputs too 124, and 134 to
-// 139 beside a profiler. The figures below are of an earlier box, where it took 116 and, all
-// cold, 124 (256 x 256 tiles: without the
+// 139 beside a profiler (256 x 256 tiles: without the
 // matrix instructions 100, without loads and reads 110, without stores 10 less, cold 20
 // less; the matrix instructions alone reach 3.5e15 to 4.1e15 on random codes).
 // Measured there, too, with stores of 64 bytes of a row (123, cold 130): tiles of
